@@ -371,6 +371,161 @@ tt_status tt_engine_get_buffer_bytes(tt_engine* e, size_t* out);
  * attention scratch).  No reference counterpart. */
 tt_status tt_engine_device_bytes(tt_engine* e, size_t* out);
 
+/* ---------------------------------------------------------------------------
+ * Paged serving of a batch of requests that share a prompt (no reference
+ * counterpart: the reference serves one sequence).  Keys and values lie
+ * uncompressed in a pool of pages of `page_size` tokens; a request's table row
+ * names its pages in token order, and a slot is page * page_size + token in
+ * page.  One step: tt_page_tables (pages, slots and positions of the step's
+ * rows), tt_qk_norm_rope (normed, rotated queries; keys and values into the
+ * slots), tt_shared_prefix_attention.
+ *
+ * All three are stream-ordered, keep nothing between calls and run on the
+ * current device, which must own every pointer.  Values that only the device
+ * sees (lengths, slots, positions, page numbers) are never used as an address
+ * outside what the host arguments allow; each entry point says what such a
+ * value does instead. */
+typedef enum { TT_DTYPE_F32 = 0, TT_DTYPE_BF16 = 1, TT_DTYPE_F16 = 2 } tt_dtype;
+
+/* Block tables and slot maps from request lengths.
+ *
+ * Request b holds ctx_lens[b] tokens (negative counts as 0) in the first
+ * ceil(ctx / page_size) entries of its table row and brings new_lens[b] more:
+ * 0 rests, -1 (or less) means that the request has ended.
+ *  - Ended requests' pages are pushed on the free stack in request order; their
+ *    table rows stay as they were.
+ *  - Then, in request order, each request pops the pages that its new tokens
+ *    need: free_pages[top-1], free_pages[top-2], ...  A request is deferred when
+ *    its last token lies beyond table_width pages, when its rows end beyond
+ *    num_rows, or when its pages and those of the requests before it (deferred
+ *    for want of pages or not, but not those that do not fit a row or the table)
+ *    exceed the stack; it then gets no page and its table row stays.
+ *  - The step's rows are the requests' new tokens, request after request.
+ *    Row i of request b: positions = ctx + i + position_offset, slots the
+ *    token's slot, row_seq = b, row_lens = ctx + i + 1.  Rows of deferred
+ *    requests and rows behind the last request: -1 in slots and row_seq, 0 in
+ *    positions and row_lens.
+ *  - seq_lens[b] = ctx + new, ctx when deferred, 0 when ended; cu_new[b] is the
+ *    first row of request b, cu_new[num_seqs] the number of rows (deferred ones
+ *    included); *deferred counts the deferred requests; *free_count_out is the
+ *    stack's new height.
+ *
+ * tables [num_seqs, table_width] int32, rows table_stride apart.  free_pages has
+ * free_capacity entries, *free_count of them on the stack (clamped to that
+ * range); pushes beyond the capacity are dropped.  free_count_out may be
+ * free_count, and seq_lens may be ctx_lens; no other outputs may overlap inputs.
+ * workspace: tt_page_tables_workspace bytes, 8-byte aligned (may be NULL when
+ * that is 0).  num_seqs = 0 writes the padding of the rows.
+ * table_width * page_size must not exceed INT32_MAX. */
+typedef struct {
+    const int32_t* ctx_lens;
+    const int32_t* new_lens;
+    int32_t* tables;
+    int32_t* free_pages;
+    const int32_t* free_count;
+    int32_t* free_count_out;
+    int32_t* seq_lens;
+    int32_t* cu_new;
+    int64_t* slots;
+    int32_t* positions;
+    int32_t* row_seq;
+    int32_t* row_lens;
+    int32_t* deferred;
+    void* workspace;
+    int64_t table_stride;
+    int32_t num_seqs, table_width, free_capacity, page_size, num_rows, position_offset;
+} tt_page_tables_args;
+size_t tt_page_tables_workspace(int num_seqs, int num_rows);
+tt_status tt_page_tables(const tt_page_tables_args* args, void* stream);
+
+/* RMS norm of each query and key head, rotation by position, and the placing of
+ * queries, keys and values, in one pass.
+ *
+ * q [num_rows, num_q_heads, head_dim], k and v [num_rows, num_kv_heads, head_dim],
+ * all of `dtype`, given by row and head strides in elements (channels
+ * contiguous), so the parts of one fused projection are taken where they lie.
+ *   y = x * rsqrt(mean(x^2) + eps) * weight      (weight NULL: y = x)
+ *   z[c] = y[c] cos[c] - y[c+h] sin[c],  z[c+h] = y[c+h] cos[c] + y[c] sin[c]
+ * for c < h = rot_dim / 2, channels from rot_dim on are y; cos and sin are rows
+ * p = positions[row] (NULL: p = row) of two [table_rows, >= h] tables.  v is
+ * copied.  Sums and products in float32, one rounding to the output's type.
+ * Queries go to q_out[row] (q_dtype).  Keys and values (kv_dtype) go to
+ * k_dst/v_dst: with slots NULL dense rows (dst_page_stride is the row stride,
+ * page_size 1); else row -> page slots[row] / page_size, token slots[row] %
+ * page_size.  A row whose slot is negative or not below num_pages * page_size
+ * is padding: nothing of it is written, its query neither.  A position outside
+ * [0, table_rows) makes the row's rotated channels NaN.
+ * Distinct rows have distinct slots.
+ *
+ * q_dtype and kv_dtype: `dtype` or TT_DTYPE_F32.  weight and the tables:
+ * `dtype` or TT_DTYPE_F32 (weight_dtype, table_dtype).  head_dim even, at most
+ * 512; rot_dim even, 0..head_dim.  q_out may be q, and dense k_dst, v_dst may be
+ * k, v, with equal strides and types; no other overlap of inputs and outputs.
+ * v and v_dst are both NULL or neither. */
+typedef struct {
+    const void *q, *k, *v;
+    void *q_out, *k_dst, *v_dst;
+    const void *q_weight, *k_weight;
+    const void *cos, *sin;
+    const void* positions;  /* int32, or int64 when positions_i64 */
+    const int64_t* slots;
+    int64_t q_row_stride, q_head_stride, k_row_stride, k_head_stride, v_row_stride, v_head_stride;
+    int64_t q_out_row_stride, q_out_head_stride;
+    int64_t k_page_stride, k_token_stride, k_dst_head_stride;
+    int64_t v_page_stride, v_token_stride, v_dst_head_stride;
+    int64_t cos_stride, sin_stride, table_rows, num_pages;
+    int32_t num_rows, num_q_heads, num_kv_heads, head_dim, rot_dim, page_size;
+    int32_t dtype, q_dtype, kv_dtype, weight_dtype, table_dtype, positions_i64;
+    float eps;
+    int32_t reserved;
+} tt_qk_norm_rope_args;
+tt_status tt_qk_norm_rope(const tt_qk_norm_rope_args* args, void* stream);
+
+/* Decode attention of a batch over a prefix that all rows share and over each
+ * row's own pages.
+ *
+ * Row r attends the prefix tokens [0, prefix_len) on the pages prefix_table
+ * names, then the tokens [0, row_lens[r]) on the pages of table row
+ * row_seq[r] (NULL: r):
+ *   out[r][h] = softmax over both of (scale * q[r][h] . k) applied to v,
+ * query head h on kv head h / (num_q_heads / num_kv_heads).  Several new tokens
+ * of one request are several rows with their own row_lens.  A row with
+ * row_seq[r] < 0 is padding and its output stays as it was; a row with nothing
+ * to attend gives zeros.  Keys and values behind a length are not used, whatever
+ * they hold.
+ *
+ * k and v: pools of num_pages pages, element (page, token, head, channel) at
+ * page * page_stride + token * token_stride + head * head_stride + channel, all
+ * strides multiples of 8 elements, bases 16-byte aligned.  page_size: a power of
+ * two from 16 to 32768.  head_dim 64 or 128.  dtype (q, k, v, out): bf16 or f16; scores,
+ * softmax and sums are float32, the weights are rounded to dtype for the second
+ * product.  q and out have row and head strides in elements (multiples of 2 for q); out
+ * may be q with equal strides.
+ * A page number outside the pool, a length beyond the table's width or below 0, a
+ * row_seq not below num_tables: nothing outside the pool or the table is read,
+ * and the rows that need it come out NaN.
+ * workspace: tt_shared_prefix_attention_workspace bytes for the same args,
+ * 16-byte aligned; not shared by calls that can overlap. */
+typedef struct {
+    const void *q, *k, *v;
+    void* out;
+    const int32_t* prefix_table;
+    const int32_t* tables;
+    const int32_t* row_lens;
+    const int32_t* row_seq;
+    void* workspace;
+    int64_t q_row_stride, q_head_stride, out_row_stride, out_head_stride;
+    int64_t k_page_stride, k_token_stride, k_head_stride;
+    int64_t v_page_stride, v_token_stride, v_head_stride;
+    int64_t table_stride;
+    int32_t num_rows, num_q_heads, num_kv_heads, head_dim, page_size, num_pages;
+    int32_t prefix_len, table_width, num_tables, dtype;
+    float scale;
+    int32_t reserved;
+} tt_shared_prefix_args;
+tt_status tt_shared_prefix_attention_workspace(const tt_shared_prefix_args* args, size_t* bytes);
+tt_status tt_shared_prefix_attention(const tt_shared_prefix_args* args, void* stream);
+
 #if defined(__GNUC__)
 #pragma GCC visibility pop
 #endif

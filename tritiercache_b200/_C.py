@@ -24,9 +24,11 @@ import torch
 
 from . import _lib
 from ._lib import check, lib
+from .paged import page_tables, qk_norm_rope, shared_prefix_attention
 
 __all__ = ["fused_attention_decode", "quantize_k_block", "quantize_v_block", "dequantize_k",
-           "dequantize_v", "TriTierCacheEngine", "engine_step_batched"]
+           "dequantize_v", "TriTierCacheEngine", "engine_step_batched", "page_tables", "qk_norm_rope",
+           "shared_prefix_attention"]
 
 _DT_BYTES = {"f32": 4, "i32": 4, "i64": 8, "u16": 2}
 _TORCH_DT = {"f32": torch.float32, "i32": torch.int32, "i64": torch.int64, "u16": torch.int16}

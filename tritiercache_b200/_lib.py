@@ -66,6 +66,8 @@ EXPORTS = [
     "tt_engine_sharded_scores_pack", "tt_engine_sharded_scores_unpack", "tt_sharded_xch_create",
     "tt_sharded_xch_open", "tt_sharded_xch_destroy", "tt_engine_step_sharded_begin_xch",
     "tt_engine_step_sharded_merge_xch",
+    "tt_page_tables_workspace", "tt_page_tables", "tt_qk_norm_rope", "tt_shared_prefix_attention_workspace",
+    "tt_shared_prefix_attention",
     "tt_engine_ingest", "tt_engine_full_count", "tt_engine_reconstruct", "tt_engine_accumulate_scores",
 ]
 
@@ -118,8 +120,15 @@ def _declare(L):
     L.tt_engine_full_count.argtypes = [vp, C.POINTER(i)]
     L.tt_engine_reconstruct.argtypes = [vp, vp, vp, vp, i, C.POINTER(i), vp]
     L.tt_engine_accumulate_scores.argtypes = [vp, vp, vp, i, i, vp]
+    # argument structs travel as packed bytes (paged.py)
+    L.tt_page_tables_workspace.argtypes = [i, i]
+    L.tt_page_tables_workspace.restype = C.c_size_t
+    L.tt_page_tables.argtypes = [vp, vp]
+    L.tt_qk_norm_rope.argtypes = [vp, vp]
+    L.tt_shared_prefix_attention_workspace.argtypes = [vp, C.POINTER(C.c_size_t)]
+    L.tt_shared_prefix_attention.argtypes = [vp, vp]
     for name in EXPORTS:
-        if name not in ("tt_last_error", "tt_version"):
+        if name not in ("tt_last_error", "tt_version", "tt_page_tables_workspace"):
             getattr(L, name).restype = C.c_int
 
 

@@ -15,7 +15,7 @@ import sys
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 PKG = os.path.dirname(HERE)
-SOURCES = ["tt_api.cu", "tt_attn.cu", "tt_engine.cu", "tt_noalloc.cu"]
+SOURCES = ["tt_api.cu", "tt_attn.cu", "tt_engine.cu", "tt_noalloc.cu", "tt_paged.cu", "tt_prefix.cu"]
 # every header in this directory (and the C ABI header) is a dependency of
 # every object: editing any of them rebuilds all sources
 HEADERS = sorted(os.path.basename(h) for h in glob.glob(os.path.join(HERE, "*.cuh"))) + \
