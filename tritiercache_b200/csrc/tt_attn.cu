@@ -762,6 +762,8 @@ static tt_status workspace(int dev, size_t floats, float** out) {
 
 static bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
+cudaError_t prefix_device_error(int clear, int* out);  // tt_prefix.cu
+
 }  // namespace tt
 
 using namespace tt;
@@ -775,7 +777,11 @@ extern "C" tt_status tt_device_error(int clear, int* out) {
     if (clear) {
         const int zero = 0;
         s = check_cuda(cudaMemcpyToSymbol(g_device_error, &zero, sizeof(int)), "tt_device_error");
+        if (s != TT_OK) return s;
     }
+    int prefix = 0;
+    s = check_cuda(prefix_device_error(clear, &prefix), "tt_device_error");
+    if (*out == 0) *out = prefix;
     return s;
 }
 

@@ -34,11 +34,12 @@ struct PrefixParams {
     int group;                   // query heads per kv head
     int head_tiles;              // tiles of 8*NB query heads per kv head
     // prefix pass: units of (kv head, tile of tile_rows rows of (row, head of the group)), the flattened
-    // (unit, KV tile) list cut into spans of `per` for the CTAs; slot = cta + unit holds a span's partial
+    // (unit, key tile) list cut into spans of `per` for the CTAs; a span's partials are in slots
+    // 2 (cta + unit) + t of 128 rows: t the half of a 256-row tile, or even and odd key tiles of a 128-row one
     int walk_prefix;             // 1: no prefix pass, the rows' pass reads the prefix too
     int tile_rows, row_tiles, kv_tiles, per;
-    float* part_o;               // [slot][tile_rows][hd]
-    float2* part_ml;             // [slot][tile_rows] (m in log2 units, l)
+    float* part_o;               // [slot][128][hd]
+    float2* part_ml;             // [slot][128] (m in log2 units, l)
 };
 
 template <typename T> __device__ __forceinline__ void mma16816(float* c, const uint32_t* a, uint32_t b0, uint32_t b1);
@@ -366,10 +367,12 @@ __global__ void __launch_bounds__(kRowWarps * 32) k_prefix_rows(const PrefixPara
             const int row = r * p.group + h0 + h, tile = row / p.tile_rows, in = row % p.tile_rows;
             const long long u = (long long)kvh * p.row_tiles + tile;
             const long long c0 = u * p.kv_tiles / p.per, c1 = ((u + 1) * p.kv_tiles - 1) / p.per;
+            const bool pair = p.tile_rows == 256;
+            const long long first = 2 * (c0 + u) + (pair ? in >> 7 : 0), past = 2 * (c1 + u) + 2;
 #pragma unroll 4
-            for (long long s = c0; s <= c1; ++s) {
-                const long long slot = (s + u) * p.tile_rows + in;
-                jn.add(p.part_ml[slot], *reinterpret_cast<const float4*>(p.part_o + slot * HD + c));
+            for (long long s = first; s < past; s += pair ? 2 : 1) {
+                const long long at = s * 128 + (in & 127);
+                jn.add(p.part_ml[at], *reinterpret_cast<const float4*>(p.part_o + at * HD + c));
             }
         }
         const float inv = jn.L == 0.f ? 0.f : 1.f / jn.L;

@@ -1,0 +1,448 @@
+// tt_prefix_shared.cuh -- the pass of tt_shared_prefix_attention over the prefix that all rows share.
+//
+// For one kv head the rows of all requests' query heads form one matrix of num_rows * group rows, so the
+// prefix is a dense attention of that matrix over prefix_len keys: GEMM-shaped work, on the tensor cores
+// (tcgen05), each K and V page read once per tile of rows.  A CTA holds two 128-row accumulators at once,
+// so that the tensor cores work for one while the softmax warps work for the other:
+//   PAIR   (more than 128 rows per kv head)  the two halves of a 256-row tile, over the same keys
+//   !PAIR  (at most 128)                     one 128-row tile, over the even and the odd key tiles
+// Per key tile of 128 tokens and accumulator t:  S_t = Q K^T (both from shared memory, into tensor memory),
+// the softmax warps read S_t (a thread a row), write P_t = 2^(S_t scale - m) over it in the pages' type,
+// and O_t += P_t V (P from tensor memory, V from shared memory).  m is a reference that is raised, and O
+// rescaled, only when a logit exceeds it by kSlack, as in the rows' pass.
+//
+// Work: units of (kv head, row tile), each kv_tiles key tiles; the flattened list is cut into equal spans,
+// one per CTA, so that every SM has the same number of tiles whatever the shape.  A span inside a unit
+// leaves one partial (m, l, O) per accumulator in the workspace, in slot 2 (cta + unit) + t, which no other
+// span has; the rows' pass joins them.
+//
+// Warps: 0 loads K and V (TMA, one box per page and 64 channels, 128-byte swizzle), 1 issues the matrix
+// instructions, 2 clears the V rows behind the prefix's end (what lies there may be NaN, and 0 * NaN is not
+// 0), 4-7 and 8-11 are the softmax of the two accumulators and load their queries.
+#pragma once
+#include <cuda.h>
+
+#include "tt_prefix_rows.cuh"
+
+namespace tt {
+
+__device__ int g_prefix_error = 0;  // a bounded wait that ran out (TT_ERR_TIMEOUT); reported by tt_device_error
+
+constexpr int kPsThreads = 384;
+constexpr int kPsTile = 128;                       // keys per tile, rows per accumulator
+constexpr long long kPsPatience = 4000000000LL;    // clocks a wait may take (about two seconds)
+
+template <int HD, bool PAIR> struct PsShape {
+    static constexpr int kSlot = kPsTile * HD * 2;                 // a K or V tile
+    static constexpr int kHalf = kPsTile * 64 * 2;                 // 64 of its channels: 128-byte rows
+    static constexpr int kQ = (PAIR ? 2 : 1) * kSlot;
+    static constexpr int kSlots = HD == 128 ? (PAIR ? 5 : 6) : 8;
+    static constexpr int kSmem = 1024 + kQ + kSlots * kSlot + 256; // alignment, tiles, barriers
+    static constexpr uint32_t kTmemO = 256;                        // S_0 S_1 in columns 0, 128; O_t behind
+};
+
+struct PsBars {  // in shared memory
+    uint64_t full[8], empty[8], q_full, s_full[2], p_ready[2], v_cut, v_fixed, drain;
+    uint32_t tmem;
+    int abort, bad;
+};
+
+__device__ __forceinline__ void bar_init(uint32_t b, uint32_t n) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(b), "r"(n) : "memory"); }
+__device__ __forceinline__ void bar_arrive(uint32_t b) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(b) : "memory"); }
+__device__ __forceinline__ void bar_expect(uint32_t b, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(b), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ bool bar_try(uint32_t b, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}"
+                 : "=r"(ok) : "r"(b), "r"(parity) : "memory");
+    return ok != 0;
+}
+// Bounded: false when it took too long here (recorded) or elsewhere in the CTA.
+__device__ __noinline__ bool bar_wait_slow(uint32_t b, uint32_t parity, volatile int* abort) {
+    const long long t0 = clock64();
+    while (clock64() - t0 < kPsPatience) {
+        if (bar_try(b, parity)) return true;
+        if (abort && *abort) return false;
+    }
+    if (abort) *abort = 1;
+    atomicCAS(&g_prefix_error, 0, (int)TT_ERR_TIMEOUT);
+    return false;
+}
+__device__ __forceinline__ bool bar_wait(uint32_t b, uint32_t parity, volatile int* abort) {
+    return bar_try(b, parity) || bar_wait_slow(b, parity, abort);
+}
+
+// The same by a whole warp, with one answer.
+__device__ __forceinline__ bool bar_wait_warp(uint32_t b, uint32_t parity, volatile int* abort) {
+    return __all_sync(~0u, bar_wait(b, parity, abort));
+}
+
+__device__ __forceinline__ void tma_load4(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, int c3, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+                 ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar) : "memory");
+}
+
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_commit(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void tc_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc) : "memory");
+}
+__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc) {
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}"
+                 ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc) : "memory");
+}
+#define TT_R4(v, i) "=r"(v[i]), "=r"(v[i + 1]), "=r"(v[i + 2]), "=r"(v[i + 3])
+#define TT_W4(v, i) "r"(v[i]), "r"(v[i + 1]), "r"(v[i + 2]), "r"(v[i + 3])
+// 32 columns of the warp's 32 lanes: v[c] is column c of this thread's lane.
+__device__ __forceinline__ void tc_ld32(uint32_t* v, uint32_t addr) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
+                 "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+                 : TT_R4(v, 0), TT_R4(v, 4), TT_R4(v, 8), TT_R4(v, 12), TT_R4(v, 16), TT_R4(v, 20), TT_R4(v, 24), TT_R4(v, 28)
+                 : "r"(addr));
+}
+__device__ __forceinline__ void tc_st32(uint32_t addr, const uint32_t* v) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+                 "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};"
+                 ::TT_W4(v, 0), TT_W4(v, 4), TT_W4(v, 8), TT_W4(v, 12), TT_W4(v, 16), TT_W4(v, 20), TT_W4(v, 24), TT_W4(v, 28),
+                   "r"(addr) : "memory");
+}
+__device__ __forceinline__ void tc_st16(uint32_t addr, const uint32_t* v) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};"
+                 ::TT_W4(v, 0), TT_W4(v, 4), TT_W4(v, 8), TT_W4(v, 12), "r"(addr) : "memory");
+}
+__device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Shared-memory operand descriptors, 128-byte swizzle.  K-major (rows of 64 channels, groups of eight rows
+// 1024 bytes apart) and MN-major (V: a token's 64 channels contiguous; groups of eight tokens 1024 bytes
+// apart, the next 64 channels `lbo` bytes on).
+__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lbo, uint32_t sbo) {
+    return (uint64_t)((addr & 0x3FFFF) >> 4) | (uint64_t)(lbo >> 4) << 16 | (uint64_t)(sbo >> 4) << 32 | 1ull << 46 | 2ull << 61;
+}
+template <typename T> constexpr uint32_t ps_idesc(int n, bool b_mn) {
+    const uint32_t fmt = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+    return 1u << 4 | fmt << 7 | fmt << 10 | (b_mn ? 1u << 16 : 0u) | (uint32_t)(n >> 3) << 17 | (uint32_t)(kPsTile >> 4) << 24;
+}
+
+// The spans of this CTA: fn(unit, first key tile, key tiles) for each, until fn returns false.
+template <typename F>
+__device__ __forceinline__ void ps_spans(const PrefixParams& p, F fn) {
+    const long long total = (long long)p.a.num_kv_heads * p.row_tiles * p.kv_tiles;
+    long long f = (long long)blockIdx.x * p.per;
+    const long long end = f + p.per < total ? f + p.per : total;
+    while (f < end) {
+        const int u = (int)(f / p.kv_tiles), k0 = (int)(f % p.kv_tiles);
+        const int n = (int)(end - f < p.kv_tiles - k0 ? end - f : p.kv_tiles - k0);
+        if (!fn(u, k0, n)) return;
+        f += n;
+    }
+}
+
+template <typename T, int HD, bool PAIR>
+__global__ void __launch_bounds__(kPsThreads, 1)
+k_prefix_shared(const PrefixParams p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
+    using S = PsShape<HD, PAIR>;
+    constexpr int kLook = PAIR ? 1 : 2;  // key tiles whose first product is issued ahead
+    extern __shared__ unsigned char raw[];
+    unsigned char* sm = reinterpret_cast<unsigned char*>(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
+    PsBars* bars = reinterpret_cast<PsBars*>(sm + S::kQ + S::kSlots * S::kSlot);
+    const uint32_t q_s = smem_addr(sm), ring = q_s + S::kQ;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const tt_shared_prefix_args& a = p.a;
+    volatile int* abort = &bars->abort;
+    const uint32_t full = smem_addr(bars->full), empty = smem_addr(bars->empty), q_full = smem_addr(&bars->q_full),
+                   s_full = smem_addr(bars->s_full), p_ready = smem_addr(bars->p_ready), v_cut = smem_addr(&bars->v_cut),
+                   v_fixed = smem_addr(&bars->v_fixed), drain = smem_addr(&bars->drain);
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < S::kSlots; ++i) {
+            bar_init(full + 8 * i, 1);
+            bar_init(empty + 8 * i, 1);
+        }
+        bar_init(q_full, PAIR ? 256 : 128);
+        for (int t = 0; t < 2; ++t) {
+            bar_init(s_full + 8 * t, 1);
+            bar_init(p_ready + 8 * t, 128);
+        }
+        bar_init(v_cut, 1);
+        bar_init(v_fixed, 32);
+        bar_init(drain, 1);
+        bars->abort = 0;
+        bars->bad = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&bars->tmem)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        tc_fence_before();
+    }
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = bars->tmem;
+    pdl_trigger();
+
+    if (warp == 0) {
+        // ---- K and V tiles into the ring, in the order the products take them
+        const int box = a.page_size < kPsTile ? a.page_size : kPsTile;  // tokens per load
+        const int boxes = kPsTile / box;
+        uint32_t it = 0;
+        ps_spans(p, [&](int u, int k0, int n) {
+            const int kvh = u / p.row_tiles;
+            const auto load = [&](const CUtensorMap* map, int tile) {
+                const int t0 = (k0 + tile) * kPsTile;
+                const int left = a.prefix_len - t0, use = left < kPsTile ? (left + box - 1) / box : boxes;
+                int page = a.num_pages;  // outside the pool: the load gives zeros
+                if (lane < use) {
+                    page = a.prefix_table[(t0 + lane * box) >> p.page_shift];
+                    if (page < 0 || page >= a.num_pages) {
+                        page = a.num_pages;
+                        *(volatile int*)&bars->bad = 1;  // before the arrival below, seen by all that depends on it
+                    }
+                }
+                const uint32_t slot = it % S::kSlots, phase = (it / S::kSlots) & 1;
+                if (!bar_wait_warp(empty + 8 * slot, phase ^ 1, abort)) return false;
+                if (lane == 0) bar_expect(full + 8 * slot, use * box * HD * 2);
+                __syncwarp();
+                if (lane < use) {
+                    const uint32_t dst = ring + slot * S::kSlot + lane * box * 128;
+                    const int row = (t0 + lane * box) & (a.page_size - 1);
+#pragma unroll
+                    for (int h = 0; h < HD / 64; ++h) tma_load4(dst + h * S::kHalf, map, h * 64, kvh, row, page, full + 8 * slot);
+                }
+                ++it;
+                return true;
+            };
+            for (int i = 0; i < kLook && i < n; ++i)
+                if (!load(&kmap, i)) return false;
+            for (int j = 0; j < n; ++j) {
+                if (!load(&vmap, j)) return false;
+                if (j + kLook < n && !load(&kmap, j + kLook)) return false;
+            }
+            return true;
+        });
+        if (*abort)  // no copy may be in flight when the CTA ends
+            for (uint32_t i = it > S::kSlots ? it - S::kSlots : 0; i < it; ++i)
+                bar_wait_slow(full + 8 * (i % S::kSlots), (i / S::kSlots) & 1, nullptr);
+    } else if (warp == 1) {
+        // ---- the matrix instructions, from one thread
+        if (lane == 0) {
+            constexpr uint32_t id_qk = ps_idesc<T>(kPsTile, false), id_pv = ps_idesc<T>(HD, true);
+            uint32_t it = 0, q_phase = 0, fix_phase = 0, p_phase[2] = {0, 0};
+            const auto slot_of = [&](uint32_t i) { return ring + (i % S::kSlots) * S::kSlot; };
+            const auto slot_full = [&](uint32_t i) { return bar_wait(full + 8 * (i % S::kSlots), (i / S::kSlots) & 1, abort); };
+            const auto qk = [&](int t, uint32_t i) {
+                const uint32_t q = q_s + (PAIR ? t * S::kSlot : 0), k = slot_of(i);
+#pragma unroll
+                for (int s = 0; s < HD / 16; ++s) {
+                    const uint32_t off = (s / 4) * S::kHalf + (s % 4) * 32;
+                    tc_mma_ss(tmem + t * 128, smem_desc(q + off, 16, 1024), smem_desc(k + off, 16, 1024), id_qk, s > 0);
+                }
+            };
+            const auto pv = [&](int t, uint32_t i, bool acc) {
+                const uint32_t v = slot_of(i);
+#pragma unroll
+                for (int s = 0; s < kPsTile / 16; ++s)
+                    tc_mma_ts(tmem + S::kTmemO + t * HD, tmem + t * 128 + s * 8, smem_desc(v + s * 2048, S::kHalf, 1024), id_pv,
+                              acc || s > 0);
+            };
+            ps_spans(p, [&](int u, int k0, int n) {
+                if (!bar_wait(q_full, q_phase, abort)) return false;
+                q_phase ^= 1;
+                tc_fence_after();
+                const bool cut = k0 + n == p.kv_tiles && a.prefix_len % kPsTile;
+                for (int i = 0; i < kLook && i < n; ++i) {
+                    if (!slot_full(it)) return false;
+                    tc_fence_after();
+                    for (int t = PAIR ? 0 : i; t < (PAIR ? 2 : i + 1); ++t) {
+                        qk(t, it);
+                        tc_commit(s_full + 8 * t);
+                    }
+                    tc_commit(empty + 8 * (it % S::kSlots));
+                    ++it;
+                }
+                for (int j = 0; j < n; ++j) {
+                    const uint32_t vi = it++, ki = it;
+                    const bool more = j + kLook < n;
+                    if (more) ++it;
+                    if (!slot_full(vi)) return false;
+                    if (cut && j == n - 1) {
+                        bar_arrive(v_cut);
+                        if (!bar_wait(v_fixed, fix_phase, abort)) return false;
+                        fix_phase ^= 1;
+                    }
+                    for (int t = PAIR ? 0 : j & 1; t < (PAIR ? 2 : (j & 1) + 1); ++t) {
+                        if (!bar_wait(p_ready + 8 * t, p_phase[t], abort)) return false;
+                        p_phase[t] ^= 1;
+                        tc_fence_after();
+                        pv(t, vi, PAIR ? j > 0 : j > 1);
+                        if (!PAIR || t == 1) tc_commit(empty + 8 * (vi % S::kSlots));
+                        if (more) {
+                            if ((!PAIR || t == 0) && !slot_full(ki)) return false;
+                            tc_fence_after();
+                            qk(t, ki);
+                            if (!PAIR || t == 1) tc_commit(empty + 8 * (ki % S::kSlots));
+                        }
+                        tc_commit(s_full + 8 * t);  // the next S_t, or the last O_t
+                    }
+                }
+                return true;
+            });
+            // every product and every arrival above has happened before the CTA gives its memory back
+            tc_commit(drain);
+            bar_wait_slow(drain, 0, nullptr);
+        }
+        __syncwarp();
+    } else if (warp == 2) {
+        // ---- V rows behind the end of the prefix
+        if (a.prefix_len % kPsTile) {
+            uint32_t loads = 0, phase = 0;
+            ps_spans(p, [&](int u, int k0, int n) {
+                loads += 2 * n;
+                if (k0 + n != p.kv_tiles) return true;
+                if (!bar_wait_warp(v_cut, phase, abort)) return false;
+                phase ^= 1;
+                const int from = a.prefix_len % kPsTile * 8;
+                unsigned char* v = sm + S::kQ + (loads - 1) % S::kSlots * S::kSlot;  // the span's last load
+                for (int x = from + lane; x < kPsTile * 8; x += 32)
+#pragma unroll
+                    for (int h = 0; h < HD / 64; ++h) *reinterpret_cast<uint4*>(v + h * S::kHalf + x * 16) = make_uint4(0, 0, 0, 0);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                bar_arrive(v_fixed);
+                return true;
+            });
+        }
+    } else if (warp >= 4) {
+        // ---- softmax: thread = row of accumulator t
+        const int t = (warp - 4) >> 2, row = threadIdx.x & 127;
+        const uint32_t lanes = tmem + ((uint32_t)(row & 96) << 16), s_col = lanes + t * 128, o_col = lanes + S::kTmemO + t * HD;
+        const int rows_all = a.num_rows * p.group;
+        const bool q16 = !(((uintptr_t)a.q & 15) | ((a.q_row_stride | a.q_head_stride) & 7));
+        uint32_t phase = 0;
+        ps_spans(p, [&](int u, int k0, int n) {
+            const int kvh = u / p.row_tiles, mine = PAIR ? n : (n - t + 1) / 2;
+            const int mrow = (u % p.row_tiles) * p.tile_rows + (PAIR ? t * kPsTile : 0) + row;
+            const bool warp_on = mrow - lane < rows_all;  // any row of this warp
+            if (PAIR || t == 0) {
+                // this row's query into the swizzled layout of the first product
+                const int r = mrow / p.group, h = kvh * p.group + mrow % p.group;
+                const uint4* src = reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + r * a.q_row_stride + h * a.q_head_stride);
+                unsigned char* dst = sm + (PAIR ? t * S::kSlot : 0) + row * 128;
+#pragma unroll 4
+                for (int c = 0; c < HD / 8; ++c) {
+                    uint4 x = make_uint4(0, 0, 0, 0);
+                    if (mrow < rows_all) {
+                        if (q16) x = src[c];
+                        else {
+                            const uint32_t* s4 = reinterpret_cast<const uint32_t*>(src + c);
+                            x = make_uint4(s4[0], s4[1], s4[2], s4[3]);
+                        }
+                    }
+                    *reinterpret_cast<uint4*>(dst + (c / 8) * S::kHalf + (((c % 8) ^ (row & 7)) << 4)) = x;
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                bar_arrive(q_full);
+            }
+            float m = -INFINITY, l = 0.f;
+            for (int i = 0; i < mine; ++i) {
+                if (!bar_wait_warp(s_full + 8 * t, phase, abort)) return false;
+                phase ^= 1;
+                tc_fence_after();
+                if (warp_on) {
+                    float s[kPsTile];
+                    uint32_t* su = reinterpret_cast<uint32_t*>(s);
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) tc_ld32(su + 32 * c, s_col + 32 * c);
+                    tc_wait_ld();
+                    const int left = a.prefix_len - (k0 + (PAIR ? i : 2 * i + t)) * kPsTile;
+                    if (left < kPsTile) {
+#pragma unroll
+                        for (int c = 0; c < kPsTile; ++c) s[c] = c < left ? s[c] : -INFINITY;
+                    }
+                    float mx[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+                    for (int c = 4; c < kPsTile; ++c) mx[c & 3] = fmaxf(mx[c & 3], s[c]);
+                    const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
+                    if (__any_sync(~0u, top > m + kSlack)) {
+                        const float nm = fmaxf(m, top);
+                        const float f = nm == m ? 1.f : m == -INFINITY ? 0.f : fast_exp2(m - nm);
+                        m = nm;
+                        l *= f;
+                        if (i > 0) {
+#pragma unroll
+                            for (int c = 0; c < HD / 32; ++c) {
+                                uint32_t o[32];
+                                tc_ld32(o, o_col + 32 * c);
+                                tc_wait_ld();
+#pragma unroll
+                                for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+                                tc_st32(o_col + 32 * c, o);
+                            }
+                        }
+                    }
+                    const float me = m == -INFINITY ? 0.f : m;
+                    float ls[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t w[16];
+#pragma unroll
+                        for (int k = 0; k < 16; ++k) {
+                            const float x = fast_exp2(fmaf(s[32 * c + 2 * k], p.scale_log2, -me));
+                            const float y = fast_exp2(fmaf(s[32 * c + 2 * k + 1], p.scale_log2, -me));
+                            ls[k & 3] += x + y;
+                            w[k] = pack2<T>(x, y);
+                        }
+                        tc_st16(s_col + 16 * c, w);
+                    }
+                    l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
+                    tc_wait_st();
+                }
+                tc_fence_before();
+                bar_arrive(p_ready + 8 * t);
+            }
+            // the span's partial
+            const long long slot = 2LL * (blockIdx.x + u) + t;
+            if (mine > 0) {
+                if (!bar_wait_warp(s_full + 8 * t, phase, abort)) return false;
+                phase ^= 1;
+                tc_fence_after();
+                if (warp_on) {
+                    float* dst = p.part_o + (slot * kPsTile + row) * HD;
+#pragma unroll
+                    for (int c = 0; c < HD / 32; ++c) {
+                        uint32_t o[32];
+                        tc_ld32(o, o_col + 32 * c);
+                        tc_wait_ld();
+                        if (mrow < rows_all) {
+#pragma unroll
+                            for (int k = 0; k < 8; ++k)
+                                *reinterpret_cast<uint4*>(dst + 32 * c + 4 * k) = make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+                        }
+                    }
+                }
+                tc_fence_before();
+            }
+            if (mrow < rows_all) p.part_ml[slot * kPsTile + row] = make_float2(m, *(volatile int*)&bars->bad ? NAN : l);
+            return true;
+        });
+        if (*abort) {
+            // a wait ran out: nothing that this CTA was to leave may be taken for a result
+            ps_spans(p, [&](int u, int k0, int n) {
+                p.part_ml[(2LL * (blockIdx.x + u) + t) * kPsTile + row] = make_float2(-INFINITY, NAN);
+                return true;
+            });
+        }
+    }
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    }
+}
+
+}  // namespace tt
