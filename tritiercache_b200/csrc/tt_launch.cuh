@@ -1,4 +1,4 @@
-// tt_launch.cuh -- launches with programmatic dependence on the kernel before and with clusters.
+// tt_launch.cuh -- launches with programmatic dependence on the kernel before.
 #pragma once
 #include <cuda_runtime.h>
 
@@ -12,23 +12,17 @@ __device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.lau
 
 template <typename... P, typename... A>
 inline cudaError_t launch(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, bool dependent,
-                          int cluster, A... args) {
+                          A... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = block;
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
-    cudaLaunchAttribute at[2];
+    cudaLaunchAttribute at[1];
     int n = 0;
     if (dependent) {
         at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
         at[n++].val.programmaticStreamSerializationAllowed = 1;
-    }
-    if (cluster > 1) {
-        at[n].id = cudaLaunchAttributeClusterDimension;
-        at[n].val.clusterDim.x = (unsigned)cluster;
-        at[n].val.clusterDim.y = 1;
-        at[n++].val.clusterDim.z = 1;
     }
     cfg.attrs = at;
     cfg.numAttrs = (unsigned)n;

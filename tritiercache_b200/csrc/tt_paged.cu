@@ -445,7 +445,7 @@ static cudaError_t launch_norm_rope(const tt_qk_norm_rope_args& a, bool vec, cud
     const int chunks = (heads + chunk - 1) / chunk;
     const long long threads = (long long)a.num_rows * chunks * G;
     const dim3 grid((unsigned)((threads + 255) / 256)), block(256);
-#define TT_NR(VV, SS) launch(k_norm_rope<T, TQ, TKV, VV, SS>, grid, block, 0, st, false, 1, a, glog, chunk, chunks)
+#define TT_NR(VV, SS) launch(k_norm_rope<T, TQ, TKV, VV, SS>, grid, block, 0, st, false, a, glog, chunk, chunks)
     if (vec) return steps <= 1 ? TT_NR(V, 1) : TT_NR(V, 2);
     return steps <= 2 ? TT_NR(1, 2) : TT_NR(1, 8);
 #undef TT_NR
@@ -491,16 +491,16 @@ tt_status tt_page_tables(const tt_page_tables_args* args, void* stream) {
     if (pt_small(a.num_seqs, a.num_rows)) {
         const int threads = a.num_seqs <= 256 * kPtItems && a.num_rows <= 1024 ? 256 : kPtThreads;
         return check_cuda(launch(k_page_scan<true>, dim3(1), dim3(threads), (3 * (size_t)a.num_seqs + 1) * sizeof(int),
-                                 st, false, 1, a), "page_tables");
+                                 st, false, a), "page_tables");
     }
     if (!a.workspace || ((uintptr_t)a.workspace & 7))
         return set_error(TT_ERR_INVALID_ARGUMENT, "page_tables: workspace is missing or not 8-byte aligned.");
-    tt_status s = check_cuda(launch(k_page_scan<false>, dim3(1), dim3(kPtThreads), 0, st, false, 1, a), "page_tables");
+    tt_status s = check_cuda(launch(k_page_scan<false>, dim3(1), dim3(kPtThreads), 0, st, false, a), "page_tables");
     if (s != TT_OK) return s;
     const int row_blocks = (int)(((long long)a.num_rows + kPrThreads * kPrRows - 1) / (kPrThreads * kPrRows));
     int seq_blocks = (a.num_seqs + kPrThreads / 32 - 1) / (kPrThreads / 32);
     seq_blocks = seq_blocks > 148 * 8 ? 148 * 8 : seq_blocks;
-    return check_cuda(launch(k_page_rows, dim3((unsigned)(row_blocks + seq_blocks)), dim3(kPrThreads), 0, st, true, 1, a,
+    return check_cuda(launch(k_page_rows, dim3((unsigned)(row_blocks + seq_blocks)), dim3(kPrThreads), 0, st, true, a,
                              row_blocks), "page_tables");
 }
 

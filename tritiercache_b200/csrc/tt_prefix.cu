@@ -10,21 +10,50 @@ static_assert(sizeof(tt_shared_prefix_args) == 208, "packed by paged.py");
 
 constexpr int kSms = 148;
 
-template <typename T, int HD, int NB>
-static cudaError_t launch_rows(const PrefixParams& p, int cluster, bool dependent, cudaStream_t st) {
-    constexpr int ST = HD == 64 ? 4 : 2;
-    const size_t smem = (size_t)kRowWarps * row_warp_bytes<HD, NB, ST>();
-    auto* kern = k_prefix_rows<T, HD, NB, ST>;
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+// All kernels ask for the whole of an SM's shared memory: the passes' CTAs share one, and an SM that has to
+// divide its memory anew between two kernels has to run dry first.
+template <typename K>
+static cudaError_t set_smem(K* kern, size_t bytes) {
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
     if (e != cudaSuccess) return e;
-    const dim3 grid((unsigned)(p.a.num_rows * cluster), (unsigned)(p.a.num_kv_heads * p.head_tiles));
-    return launch(kern, grid, dim3(kRowWarps * 32), smem, st, dependent, cluster, p);
+    return cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+}
+
+template <typename T, int HD, int NB>
+static cudaError_t launch_rows(const PrefixParams& p, const CUtensorMap& km, const CUtensorMap& vm, cudaStream_t st) {
+    constexpr int ST = HD == 64 ? 4 : 2;
+    constexpr size_t smem = row_smem<HD, NB, ST>();
+    auto* kern = k_prefix_rows<T, HD, NB, ST>;
+    const cudaError_t e = set_smem(kern, smem);
+    if (e != cudaSuccess) return e;
+    const dim3 grid((unsigned)(p.a.num_rows * p.splits), (unsigned)(p.a.num_kv_heads * p.head_tiles));
+    return launch(kern, grid, dim3(kRowWarps * 32), smem, st, !p.walk_prefix, p, km, vm);
 }
 
 template <typename T>
-static cudaError_t launch_rows_t(const PrefixParams& p, int nb, int cluster, bool dependent, cudaStream_t st) {
-    if (p.a.head_dim == 64) return nb == 1 ? launch_rows<T, 64, 1>(p, cluster, dependent, st) : launch_rows<T, 64, 2>(p, cluster, dependent, st);
-    return nb == 1 ? launch_rows<T, 128, 1>(p, cluster, dependent, st) : launch_rows<T, 128, 2>(p, cluster, dependent, st);
+static cudaError_t launch_rows_t(const PrefixParams& p, const CUtensorMap& km, const CUtensorMap& vm, cudaStream_t st) {
+    const bool one = p.group <= 8;
+    if (p.a.head_dim == 64) return one ? launch_rows<T, 64, 1>(p, km, vm, st) : launch_rows<T, 64, 2>(p, km, vm, st);
+    return one ? launch_rows<T, 128, 1>(p, km, vm, st) : launch_rows<T, 128, 2>(p, km, vm, st);
+}
+
+template <typename T, int HD, int W>
+static cudaError_t launch_join_w(const PrefixParams& p, cudaStream_t st) {
+    const cudaError_t e = set_smem(k_prefix_join<T, HD, W>, 0);
+    if (e != cudaSuccess) return e;
+    const long long warps = (long long)p.a.num_rows * p.a.num_q_heads * W;
+    return launch(k_prefix_join<T, HD, W>, dim3((unsigned)((warps + kJoinWarps - 1) / kJoinWarps)), dim3(kJoinWarps * 32), 0, st, true, p);
+}
+template <typename T, int HD>
+static cudaError_t launch_join(const PrefixParams& p, cudaStream_t st) {
+    // a warp loads eight partials at once
+    const int n = p.splits + (p.walk_prefix ? 0 : (p.kv_tiles / p.per + 1) * (p.tile_rows == kPsTile ? 2 : 1));
+    return n <= 8 ? launch_join_w<T, HD, 1>(p, st) : n <= 16 ? launch_join_w<T, HD, 2>(p, st)
+         : n <= 32 ? launch_join_w<T, HD, 4>(p, st) : launch_join_w<T, HD, 8>(p, st);
+}
+template <typename T>
+static cudaError_t launch_join_t(const PrefixParams& p, cudaStream_t st) {
+    return p.a.head_dim == 64 ? launch_join<T, 64>(p, st) : launch_join<T, 128>(p, st);
 }
 
 static tt_status check_prefix(const tt_shared_prefix_args* args) {
@@ -39,8 +68,8 @@ static tt_status check_prefix(const tt_shared_prefix_args* args) {
         return set_error(TT_ERR_UNSUPPORTED, "shared_prefix_attention: dtype must be bf16 or f16.");
     if (a.page_size < 16 || a.page_size > 32768 || (a.page_size & (a.page_size - 1)))
         return set_error(TT_ERR_UNSUPPORTED, "shared_prefix_attention: page_size must be a power of two from 16 to 32768.");
-    if (a.num_pages < 0 || a.prefix_len < 0 || a.table_width < 0 || a.num_tables < 0)
-        return set_error(TT_ERR_INVALID_ARGUMENT, "shared_prefix_attention: sizes must be non-negative.");
+    if (a.num_pages <= 0 || a.prefix_len < 0 || a.table_width < 0 || a.num_tables < 0)
+        return set_error(TT_ERR_INVALID_ARGUMENT, "shared_prefix_attention: sizes must be non-negative, num_pages positive.");
     if ((long long)a.table_width * a.page_size > INT_MAX)
         return set_error(TT_ERR_UNSUPPORTED, "shared_prefix_attention: table_width * page_size must not exceed 2^31 - 1.");
     if (!a.row_seq && a.num_tables < a.num_rows)
@@ -54,19 +83,22 @@ static tt_status check_prefix(const tt_shared_prefix_args* args) {
         return set_error(TT_ERR_UNSUPPORTED, "shared_prefix_attention: strides of k and v must be multiples of 8 elements.");
     if ((a.q_row_stride | a.q_head_stride) & 1)
         return set_error(TT_ERR_UNSUPPORTED, "shared_prefix_attention: strides of q must be multiples of 2 elements.");
+    if (((long long)a.num_rows * a.num_q_heads / kPsTile + a.num_q_heads) * (a.prefix_len / kPsTile + 1) > INT_MAX)
+        return set_error(TT_ERR_UNSUPPORTED, "shared_prefix_attention: rows times prefix_len too large for one call.");
     if (a.num_rows == 0) return TT_OK;
     if (!a.q || !a.out || !a.row_lens || (a.prefix_len > 0 && !a.prefix_table) ||
-        (a.num_tables > 0 && a.table_width > 0 && !a.tables) || (a.num_pages > 0 && (!a.k || !a.v)))
+        (a.num_tables > 0 && a.table_width > 0 && !a.tables) || !a.k || !a.v)
         return set_error(TT_ERR_INVALID_ARGUMENT, "shared_prefix_attention: null pointer argument.");
     if (((uintptr_t)a.k & 15) || ((uintptr_t)a.v & 15) || ((uintptr_t)a.q & 3))
         return set_error(TT_ERR_UNSUPPORTED, "shared_prefix_attention: k and v must be 16-byte aligned, q 4-byte aligned.");
     return TT_OK;
 }
 
-static int prefix_ctas(const PrefixParams& p) {
-    const long long total = (long long)p.a.num_kv_heads * p.row_tiles * p.kv_tiles;
-    return (int)((total + p.per - 1) / p.per);
+static int prefix_groups(const PrefixParams& p) { return (int)(((long long)p.units * p.kv_tiles + p.per - 1) / p.per); }
+static size_t prefix_slots(const PrefixParams& p) {
+    return p.walk_prefix ? 0 : 2 * ((size_t)prefix_groups(p) + (size_t)p.units) * p.lanes;
 }
+static size_t own_slots(const PrefixParams& p) { return p.join ? (size_t)p.splits * p.a.num_rows * p.a.num_q_heads : 0; }
 
 static PrefixParams plan_prefix(const tt_shared_prefix_args& a) {
     PrefixParams p = {};
@@ -77,25 +109,35 @@ static PrefixParams plan_prefix(const tt_shared_prefix_args& a) {
     p.head_tiles = p.group <= 8 ? 1 : (p.group + 15) / 16;
     // One row has nobody to share with.  The prefix pass takes its maxima before the scale, so the scale must
     // not turn them round.
-    p.walk_prefix = a.num_rows < 2 || a.prefix_len == 0 || !(a.scale > 0.f) || a.num_pages == 0;
+    p.walk_prefix = a.num_rows < 2 || a.prefix_len == 0 || !(a.scale > 0.f);
     if (!p.walk_prefix) {
         const int rows = a.num_rows * p.group;
         p.tile_rows = rows > kPsTile ? 2 * kPsTile : kPsTile;
         p.row_tiles = (rows + p.tile_rows - 1) / p.tile_rows;
         p.kv_tiles = (a.prefix_len + kPsTile - 1) / kPsTile;
-        const long long total = (long long)a.num_kv_heads * p.row_tiles * p.kv_tiles;
-        p.per = (int)((total + kSms - 1) / kSms);
+        // CTA groups over all row tiles of a kv head, unless they would leave more than a tenth of the SMs idle
+        p.lanes = kSms / p.row_tiles * p.row_tiles * 10 >= kSms * 9 ? p.row_tiles : 1;
+        p.units = a.num_kv_heads * (p.row_tiles / p.lanes);
+        const long long total = (long long)p.units * p.kv_tiles, groups = kSms / p.lanes;
+        p.per = (int)((total + groups - 1) / groups);
+        // one 128-row tile: a span of one key tile would leave its second accumulator without work
+        if (p.tile_rows == kPsTile && p.per < 2) p.per = 2;
     }
+    // CTAs of the rows' pass per row and head tile: two for each SM in all, if that leaves a warp two groups
+    const long long tokens = (long long)a.table_width * a.page_size + (p.walk_prefix ? a.prefix_len : 0);
+    const long long units = (long long)a.num_rows * a.num_kv_heads * p.head_tiles;
+    const long long most = tokens / (kRowWarps * kGroup * 2), fit = 2 * kSms / units;
+    p.splits = (int)(most < fit ? most : fit);
+    if (p.splits < 1) p.splits = 1;
+    p.join = p.splits > 1 || !p.walk_prefix;
     return p;
 }
 
 static size_t prefix_workspace(const PrefixParams& p) {
-    if (p.walk_prefix) return 0;
-    const size_t slots = 2 * ((size_t)prefix_ctas(p) + (size_t)p.a.num_kv_heads * p.row_tiles);
-    return slots * kPsTile * (p.a.head_dim * sizeof(float) + sizeof(float2));
+    return (prefix_slots(p) * kPsTile + own_slots(p)) * (p.a.head_dim * sizeof(float) + sizeof(float2));
 }
 
-// The pool as [page][token][head][channel] boxes of 64 channels and up to 128 tokens of one head.
+// The pool in boxes of 64 channels and `tokens` tokens of one head.
 using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                               const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                               CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -113,12 +155,12 @@ static EncodeFn encode_fn() {
     return fn;
 }
 static bool encode_pool(CUtensorMap* map, const tt_shared_prefix_args& a, const void* base, int64_t page, int64_t token,
-                        int64_t head) {
+                        int64_t head, int tokens) {
     const EncodeFn fn = encode_fn();
     if (!fn) return false;
     const cuuint64_t dims[4] = {(cuuint64_t)a.head_dim, (cuuint64_t)a.num_kv_heads, (cuuint64_t)a.page_size, (cuuint64_t)a.num_pages};
     const cuuint64_t strides[3] = {(cuuint64_t)head * 2, (cuuint64_t)token * 2, (cuuint64_t)page * 2};
-    const cuuint32_t box[4] = {64, 1, (cuuint32_t)(a.page_size < kPsTile ? a.page_size : kPsTile), 1};
+    const cuuint32_t box[4] = {64, 1, (cuuint32_t)tokens, 1};
     const cuuint32_t one[4] = {1, 1, 1, 1};
     return fn(map, a.dtype == TT_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
               const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
@@ -130,9 +172,9 @@ static cudaError_t launch_shared(const PrefixParams& p, const CUtensorMap& km, c
     using S = PsShape<HD, PAIR>;
     static_assert(sizeof(PsBars) <= 256 && S::kSmem <= 227 * 1024 && S::kSlots <= 8, "shared memory of the prefix pass");
     auto* kern = k_prefix_shared<T, HD, PAIR>;
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
+    const cudaError_t e = set_smem(kern, S::kSmem);
     if (e != cudaSuccess) return e;
-    return launch(kern, dim3((unsigned)prefix_ctas(p)), dim3(kPsThreads), S::kSmem, st, false, 1, p, km, vm);
+    return launch(kern, dim3((unsigned)(prefix_groups(p) * p.lanes)), dim3(kPsThreads), S::kSmem, st, false, p, km, vm);
 }
 template <typename T>
 static cudaError_t launch_shared_t(const PrefixParams& p, const CUtensorMap& km, const CUtensorMap& vm, cudaStream_t st) {
@@ -169,34 +211,36 @@ tt_status tt_shared_prefix_attention(const tt_shared_prefix_args* args, void* st
     if (s != TT_OK) return s;
     if (args->num_rows == 0) return TT_OK;
     PrefixParams p = plan_prefix(*args);
-    const bool bf = args->dtype == TT_DTYPE_BF16;
+    const tt_shared_prefix_args& a = p.a;
+    const bool bf = a.dtype == TT_DTYPE_BF16;
     const cudaStream_t st = (cudaStream_t)stream;
-    if (!p.walk_prefix) {
-        if (!args->workspace || ((uintptr_t)args->workspace & 15))
+    const auto encode = [&](CUtensorMap* km, CUtensorMap* vm, int tokens) {
+        return encode_pool(km, a, a.k, a.k_page_stride, a.k_token_stride, a.k_head_stride, tokens) &&
+               encode_pool(vm, a, a.v, a.v_page_stride, a.v_token_stride, a.v_head_stride, tokens);
+    };
+    if (prefix_workspace(p)) {
+        if (!a.workspace || ((uintptr_t)a.workspace & 15))
             return set_error(TT_ERR_INVALID_ARGUMENT, "shared_prefix_attention: workspace is missing or not 16-byte aligned.");
-        const tt_shared_prefix_args& a = p.a;
-        CUtensorMap km, vm;
-        // strides that a tensor map does not take (an expanded pool): the rows' pass reads the prefix itself
-        if (!encode_pool(&km, a, a.k, a.k_page_stride, a.k_token_stride, a.k_head_stride) ||
-            !encode_pool(&vm, a, a.v, a.v_page_stride, a.v_token_stride, a.v_head_stride)) {
-            p.walk_prefix = 1;
-        } else {
-            p.part_o = static_cast<float*>(args->workspace);
-            const size_t slots = 2 * ((size_t)prefix_ctas(p) + (size_t)a.num_kv_heads * p.row_tiles);
-            p.part_ml = reinterpret_cast<float2*>(p.part_o + slots * kPsTile * a.head_dim);
-            const tt_status e = check_cuda(bf ? launch_shared_t<__nv_bfloat16>(p, km, vm, st) : launch_shared_t<__half>(p, km, vm, st),
-                                           "shared_prefix_attention");
-            if (e != TT_OK) return e;
-        }
+        const size_t slots = prefix_slots(p) * kPsTile;
+        p.part_o = static_cast<float*>(a.workspace);
+        p.own_o = p.part_o + slots * a.head_dim;
+        p.part_ml = reinterpret_cast<float2*>(p.own_o + own_slots(p) * a.head_dim);
+        p.own_ml = p.part_ml + slots;
     }
-    // CTAs per row and head tile: enough for the GPU, and no more than leaves a warp a few groups
-    const long long tokens = (long long)args->table_width * args->page_size + (p.walk_prefix ? args->prefix_len : 0);
-    const long long units = (long long)args->num_rows * args->num_kv_heads * p.head_tiles;
-    int cluster = 1;
-    while (cluster < 8 && units * cluster < 2 * kSms && tokens > (long long)cluster * kRowWarps * kGroup * 2) cluster *= 2;
-    const int nb = p.group <= 8 ? 1 : 2;
-    return check_cuda(bf ? launch_rows_t<__nv_bfloat16>(p, nb, cluster, !p.walk_prefix, st)
-                         : launch_rows_t<__half>(p, nb, cluster, !p.walk_prefix, st), "shared_prefix_attention");
+    CUtensorMap km, vm;
+    if (!p.walk_prefix) {
+        if (!encode(&km, &vm, a.page_size < kPsTile ? a.page_size : kPsTile))
+            return set_error(TT_ERR_UNSUPPORTED, "shared_prefix_attention: no tensor map takes the strides of k and v.");
+        const tt_status e = check_cuda(bf ? launch_shared_t<__nv_bfloat16>(p, km, vm, st) : launch_shared_t<__half>(p, km, vm, st),
+                                       "shared_prefix_attention");
+        if (e != TT_OK) return e;
+    }
+    if (!encode(&km, &vm, kGroup))
+        return set_error(TT_ERR_UNSUPPORTED, "shared_prefix_attention: no tensor map takes the strides of k and v.");
+    const tt_status e = check_cuda(bf ? launch_rows_t<__nv_bfloat16>(p, km, vm, st) : launch_rows_t<__half>(p, km, vm, st),
+                                   "shared_prefix_attention");
+    if (e != TT_OK || !p.join) return e;
+    return check_cuda(bf ? launch_join_t<__nv_bfloat16>(p, st) : launch_join_t<__half>(p, st), "shared_prefix_attention");
 }
 
 }  // extern "C"

@@ -1,8 +1,8 @@
 // tt_prefix_rows.cuh -- the pass of tt_shared_prefix_attention over each row's own pages, which also
 // joins what the prefix pass left.
 //
-// One cluster of C CTAs per (row, kv head, tile of up to 8*NB query heads).  Its 4*C warps take the row's
-// tokens in groups of 16 (a group never crosses a page), warp w groups w, w+4C, ...; each warp keeps its
+// `splits` CTAs per (row, kv head, tile of up to 8*NB query heads).  Their 4*splits warps take the row's
+// tokens in groups of 16 (a group never crosses a page), warp w groups w, w+4*splits, ...; each warp keeps its
 // own cp.async pipeline of K and V groups, so no warp waits for another before the end.  Per group, with
 // mma.sync m16n8k16 and tokens along M, because a row has few query heads and 16 tokens:
 //   S^T[16 x 8] = K[16 x hd] Q^T[hd x 8]         (K by ldmatrix, Q^T in registers)
@@ -11,11 +11,14 @@
 // m is a reference, not the maximum: it is raised (and O, l rescaled) only when a logit exceeds it by
 // kSlack, so the cross-lane maximum and the rescale run once or twice a row instead of once a group;
 // weights stay below 2^kSlack and every sum is float32.
-// At the end the warps' (m, l, O) meet in shared memory, the CTAs' through the cluster's, and the prefix
-// pass's partials from the workspace: one output, no further launch.
+// At the end the warps' (m, l, O) meet in shared memory, and k_prefix_join joins what the splits and the prefix
+// pass left.  (A row's splits as a thread-block cluster joined through distributed shared memory, and the rows'
+// CTAs joining the prefix pass's partials themselves, cost more: the CTAs wait for the prefix pass, where they
+// could run beside it, its time being the tensor cores' and theirs the memory's.)
 //
 // Bound: HBM (the row's K and V are read once, by one cluster).
 #pragma once
+#include <cuda.h>
 #include <cuda_bf16.h>
 
 #include "tt_common.cuh"
@@ -27,19 +30,29 @@ constexpr float kSlack = 8.f;    // log2 units a logit may exceed the reference 
 constexpr int kRowWarps = 4;
 constexpr int kGroup = 16;       // tokens per warp step
 
+constexpr long long kPatience = 4000000000LL;  // clocks that a wait may take (about two seconds)
+
+__device__ int g_prefix_error = 0;  // a wait that ran out (TT_ERR_TIMEOUT); reported by tt_device_error
+
 struct PrefixParams {
     tt_shared_prefix_args a;
     float scale_log2;            // scale * log2(e)
     int page_shift;
     int group;                   // query heads per kv head
     int head_tiles;              // tiles of 8*NB query heads per kv head
-    // prefix pass: units of (kv head, tile of tile_rows rows of (row, head of the group)), the flattened
-    // (unit, key tile) list cut into spans of `per` for the CTAs; a span's partials are in slots
-    // 2 (cta + unit) + t of 128 rows: t the half of a 256-row tile, or even and odd key tiles of a 128-row one
+    int splits;                  // CTAs per row and head tile in the rows' pass
+    // prefix pass: a unit is a kv head and one tile of tile_rows rows of its (row, head of the group) matrix, or
+    // with lanes = row_tiles all its tiles at once, one CTA of a group of `lanes` each; the flattened (unit, key
+    // tile) list is cut into spans of `per`, one per CTA group.  A span's partials are in slots
+    // 2 ((group + unit) lanes + lane) + t of 128 rows: t is the half of a 256-row tile, or even and odd key tiles
+    // of a 128-row one
     int walk_prefix;             // 1: no prefix pass, the rows' pass reads the prefix too
-    int tile_rows, row_tiles, kv_tiles, per;
+    int tile_rows, row_tiles, lanes, units, kv_tiles, per;
     float* part_o;               // [slot][128][hd]
     float2* part_ml;             // [slot][128] (m in log2 units, l)
+    int join;                    // 1: the rows' pass leaves partials [splits][num_rows][num_q_heads] for k_prefix_join; 0: outputs
+    float* own_o;
+    float2* own_ml;
 };
 
 template <typename T> __device__ __forceinline__ void mma16816(float* c, const uint32_t* a, uint32_t b0, uint32_t b1);
@@ -91,81 +104,180 @@ __device__ __forceinline__ uint32_t movm_t(uint32_t x) {
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
-// 16 bytes to shared memory, zeros when !live (nothing is read then).
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool live) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+// Barriers in shared memory
+__device__ __forceinline__ void bar_init(uint32_t b, uint32_t n) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(b), "r"(n) : "memory"); }
+__device__ __forceinline__ void bar_arrive(uint32_t b) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(b) : "memory"); }
+__device__ __forceinline__ void bar_expect(uint32_t b, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(b), "r"(bytes) : "memory");
 }
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
-__device__ __forceinline__ uint32_t cluster_rank() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
+__device__ __forceinline__ bool bar_try(uint32_t b, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}"
+                 : "=r"(ok) : "r"(b), "r"(parity) : "memory");
+    return ok != 0;
 }
-__device__ __forceinline__ uint32_t cluster_size() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ uint32_t map_rank(uint32_t addr, uint32_t rank) {
-    uint32_t r;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
-    return r;
-}
-__device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
-    float4 v;
-    asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
-    return v;
-}
-__device__ __forceinline__ float2 ld_cluster2(uint32_t addr) {
-    float2 v;
-    asm volatile("ld.shared::cluster.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
-    return v;
-}
-
-// A running join of partials (m, l, O): adds one of weight 2^(m - M).
-struct Join {
-    float M = -INFINITY, L = 0.f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    __device__ __forceinline__ void add(float2 ml, float4 x) {
-        // an empty partial (m = -inf) has l = 0 and must not bring 2^(-inf + inf); a NaN l passes through
-        if (ml.x == -INFINITY && ml.y == 0.f) return;
-        const float n = fmaxf(M, ml.x), f = M == -INFINITY ? 0.f : fast_exp2(M - n);
-        const float w = ml.x == -INFINITY ? 1.f : fast_exp2(ml.x - n);
-        L = L * f + ml.y * w;
-        o.x = o.x * f + x.x * w;
-        o.y = o.y * f + x.y * w;
-        o.z = o.z * f + x.z * w;
-        o.w = o.w * f + x.w * w;
-        M = n;
+// Bounded: false when it took too long here (recorded) or elsewhere in the CTA.
+__device__ __noinline__ bool bar_wait_slow(uint32_t b, uint32_t parity, volatile int* abort) {
+    const long long t0 = clock64();
+    while (clock64() - t0 < kPatience) {
+        if (bar_try(b, parity)) return true;
+        if (abort && *abort) return false;
     }
-};
+    if (abort) *abort = 1;
+    atomicCAS(&g_prefix_error, 0, (int)TT_ERR_TIMEOUT);
+    return false;
+}
+__device__ __forceinline__ bool bar_wait(uint32_t b, uint32_t parity, volatile int* abort) {
+    return bar_try(b, parity) || bar_wait_slow(b, parity, abort);
+}
+
+// The same by a whole warp, with one answer.
+__device__ __forceinline__ bool bar_wait_warp(uint32_t b, uint32_t parity, volatile int* abort) {
+    return __all_sync(~0u, bar_wait(b, parity, abort));
+}
+
+// A box of the pool: channel, head, token in page, page.  Outside the pool it is zeros.
+__device__ __forceinline__ void tma_load4(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, int c3, uint32_t bar,
+                                          uint64_t policy) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%2, "
+                 "%3, %4, %5}], [%6], %7;"
+                 ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar), "l"(policy) : "memory");
+}
+__device__ __forceinline__ uint64_t policy_evict_first() {
+    uint64_t p;
+    asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(p));
+    return p;
+}
+__device__ __forceinline__ uint64_t policy_evict_last() {
+    uint64_t p;
+    asm volatile("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(p));
+    return p;
+}
+
+// A warp's join of n partials (m, l, O) of one row and query head, lane i taking channels i*HD/32 on: the
+// weights first (a lane a partial), then the O rows, whose loads wait for nothing.  ml(i) gives (m, l), o(i)
+// the address of O.  An empty partial (m = -inf, l = 0) has no O; l = NaN marks a failed one and stays.
+template <int HD, typename ML, typename O>
+__device__ __forceinline__ void join_partials(int n, ML ml, O o, float& M, float& L, float* acc) {
+    constexpr int C = HD / 32;
+    const int lane = threadIdx.x & 31;
+    M = -INFINITY;
+    for (int i = lane; i < n; i += 32) M = fmaxf(M, ml(i).x);
+#pragma unroll
+    for (int d = 16; d; d >>= 1) M = fmaxf(M, __shfl_xor_sync(~0u, M, d));
+    L = 0.f;
+#pragma unroll
+    for (int c = 0; c < C; ++c) acc[c] = 0.f;
+    for (int base = 0; base < n; base += 32) {
+        float w = 0.f;
+        if (base + lane < n) {
+            const float2 x = ml(base + lane);
+            w = M == -INFINITY ? 0.f : fast_exp2(x.x - M);
+            L += w * x.y;
+        }
+        const int m = min(32, n - base);
+#pragma unroll 8
+        for (int j = 0; j < m; ++j) {
+            const float f = __shfl_sync(~0u, w, j);
+            const float* p = o(base + j) + lane * C;
+            float x[C];
+            if constexpr (C == 4) *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(p);
+            else *reinterpret_cast<float2*>(x) = *reinterpret_cast<const float2*>(p);
+#pragma unroll
+            for (int c = 0; c < C; ++c) acc[c] += f != 0.f ? f * x[c] : 0.f;
+        }
+    }
+#pragma unroll
+    for (int d = 16; d; d >>= 1) L += __shfl_xor_sync(~0u, L, d);
+}
+
+template <typename T, int HD>
+__device__ __forceinline__ void store_out(const PrefixParams& p, float L, const float* acc, int r, int head) {
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+    T* out = static_cast<T*>(p.a.out) + r * p.a.out_row_stride + (long long)head * p.a.out_head_stride + (threadIdx.x & 31) * (HD / 32);
+#pragma unroll
+    for (int c = 0; c < HD / 32; ++c) out[c] = from_f32<T>(acc[c] * inv);
+}
+
+// The join of the two passes: W warps a (row, query head), each a W-th of its partials, so that their loads
+// are in flight together.
+constexpr int kJoinWarps = 8;
+
+template <typename T, int HD, int W>
+__global__ void __launch_bounds__(kJoinWarps * 32) k_prefix_join(const PrefixParams p) {
+    __shared__ __align__(16) float so[kJoinWarps][HD];
+    __shared__ float2 sml[kJoinWarps];
+    const tt_shared_prefix_args& a = p.a;
+    const int warp = threadIdx.x >> 5, sub = warp % W;
+    const long long rh = (long long)blockIdx.x * (kJoinWarps / W) + warp / W, all = (long long)a.num_rows * a.num_q_heads;
+    const int r = (int)(rh / a.num_q_heads), head = (int)(rh % a.num_q_heads);
+    const bool on = rh < all && !(a.row_seq && a.row_seq[r] < 0);
+    // the prefix pass's partials of this row: np of them, `step` slots of 128 rows apart from `first`
+    long long first = 0, step = 0;
+    int np = 0;
+    if (!p.walk_prefix) {
+        const int kvh = head / p.group, row = r * p.group + head % p.group;
+        const int tile = row / p.tile_rows, in = row % p.tile_rows, lane = p.lanes > 1 ? tile : 0;
+        const bool pair = p.tile_rows == 256;
+        const int u = p.lanes > 1 ? kvh : kvh * p.row_tiles + tile;
+        const int g0 = u * p.kv_tiles / p.per, g1 = ((u + 1) * p.kv_tiles - 1) / p.per;
+        // even and odd key tiles are neighbours (!pair has one row tile, so one lane)
+        first = (2 * ((long long)(g0 + u) * p.lanes + lane) + (pair ? in >> 7 : 0)) * 128 + (in & 127);
+        step = (pair ? 2 * p.lanes : 1) * 128;
+        np = (g1 - g0 + 1) * (pair ? 1 : 2);
+    }
+    const int n = on ? (p.splits + np - sub + W - 1) / W : 0;
+    pdl_wait();
+    float M, L, acc[HD / 32];
+    join_partials<HD>(n,
+                      [&](int k) {
+                          const int i = k * W + sub;
+                          return *(i < p.splits ? p.own_ml + (i * all + rh) : p.part_ml + (first + (i - p.splits) * step));
+                      },
+                      [&](int k) {
+                          const int i = k * W + sub;
+                          return i < p.splits ? p.own_o + (i * all + rh) * HD : p.part_o + (first + (i - p.splits) * step) * HD;
+                      },
+                      M, L, acc);
+    if constexpr (W > 1) {
+#pragma unroll
+        for (int c = 0; c < HD / 32; ++c) so[warp][(threadIdx.x & 31) * (HD / 32) + c] = acc[c];
+        if ((threadIdx.x & 31) == 0) sml[warp] = make_float2(M, L);
+        __syncthreads();
+        if (sub) return;
+        join_partials<HD>(W, [&](int k) { return sml[warp + k]; }, [&](int k) { return so[warp + k]; }, M, L, acc);
+    }
+    if (on) store_out<T, HD>(p, L, acc, r, head);
+}
 
 template <int HD, int NB> constexpr int row_out_bytes() { return 8 * NB * HD * 4 + 8 * NB * 8; }  // one warp's O and (m, l)
 template <int HD, int NB, int ST> constexpr int row_warp_bytes() {
-    return ST * 2 * kGroup * HD * 2 > row_out_bytes<HD, NB>() ? ST * 2 * kGroup * HD * 2 : row_out_bytes<HD, NB>();
+    static_assert(ST * 2 * kGroup * HD * 2 >= row_out_bytes<HD, NB>(), "the partials take the stages' place");
+    return ST * 2 * kGroup * HD * 2;
 }
+template <int HD, int NB, int ST> constexpr int row_smem() { return kRowWarps * (row_warp_bytes<HD, NB, ST>() + 2 * ST * 8); }
 
 template <typename T, int HD, int NB, int ST>
-__global__ void __launch_bounds__(kRowWarps * 32) k_prefix_rows(const PrefixParams p) {
-    extern __shared__ __align__(128) unsigned char sm[];
-    constexpr int KS = HD / 16, CH = HD / 8;          // k-steps, 16-byte chunks of a token's row
-    constexpr int kTile = kGroup * HD * 2;            // bytes of a K (or V) group
+__global__ void __launch_bounds__(kRowWarps * 32, 4)
+k_prefix_rows(const PrefixParams p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
+    extern __shared__ __align__(1024) unsigned char sm[];
+    constexpr int KS = HD / 16;                       // k-steps of the first product
+    constexpr int kTile = kGroup * HD * 2;            // bytes of a K (or V) group: HD / 64 boxes of 16 x 128
     constexpr int kWarp = row_warp_bytes<HD, NB, ST>();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t rank = cluster_rank(), C = cluster_size();
-    const int r = blockIdx.x / C;
+    const int r = blockIdx.x / p.splits, split = blockIdx.x % p.splits;
     const int kvh = blockIdx.y / p.head_tiles, h0 = (blockIdx.y % p.head_tiles) * 8 * NB;
     const int heads = min(8 * NB, p.group - h0);      // query heads of this tile
     const tt_shared_prefix_args& a = p.a;
 
+    // This grid runs beside the prefix pass and waits for nothing of it, but must not end before it does, for the
+    // join waits for this grid alone: the last CTA sees to that.
+    const bool last = blockIdx.x == gridDim.x - 1 && blockIdx.y == gridDim.y - 1;
+    pdl_trigger();
+
     const int seq = a.row_seq ? a.row_seq[r] : r;
-    if (seq < 0) {  // padding; the wait keeps this grid from ending before the prefix pass
-        pdl_wait();
+    if (seq < 0) {  // padding
+        if (last) pdl_wait();
         return;
     }
     int len = a.row_lens[r];
@@ -177,45 +289,44 @@ __global__ void __launch_bounds__(kRowWarps * 32) k_prefix_rows(const PrefixPara
     const int pre_groups = p.walk_prefix ? (a.prefix_len + kGroup - 1) / kGroup : 0;
     const int groups = pre_groups + (len + kGroup - 1) / kGroup;
     const int* own = a.tables + (long long)(bad ? 0 : seq) * a.table_stride;
-    const int step = kRowWarps * C, g0 = rank * kRowWarps + warp;
+    const int step = kRowWarps * p.splits, g0 = split * kRowWarps + warp;
     const int gpp = p.page_shift - 4;                 // log2 groups per page
 
-    // first token of group g, its page (-1 none) and the tokens that count
-    const auto page_of = [&](int g) {
-        if (g >= groups) return -1;
-        return g < pre_groups ? a.prefix_table[g >> gpp] : own[(g - pre_groups) >> gpp];
-    };
     const uint32_t base = smem_addr(sm) + warp * kWarp;
-    const T* kp = static_cast<const T*>(a.k) + (long long)kvh * a.k_head_stride;
-    const T* vp = static_cast<const T*>(a.v) + (long long)kvh * a.v_head_stride;
-    const auto issue = [&](int g, int page, int stage) {
-        if (g < groups) {
-            const int t0 = (g < pre_groups ? g : g - pre_groups) * kGroup;
-            const int n = (g < pre_groups ? a.prefix_len : len) - t0;
-            const bool ok = page >= 0 && page < a.num_pages;
-            bad |= !ok;
-            const long long pg = ok ? page : 0;
-            const int in_page = t0 & (a.page_size - 1);
-            const T* ks = kp + pg * a.k_page_stride + in_page * a.k_token_stride;
-            const T* vs = vp + pg * a.v_page_stride + in_page * a.v_token_stride;
-            const uint32_t kd = base + stage * 2 * kTile, vd = kd + kTile;
+    const uint32_t bars = smem_addr(sm) + kRowWarps * kWarp + warp * 2 * ST * 8;  // K of each stage, V of each stage
+    if (lane == 0) {
+        for (int i = 0; i < 2 * ST; ++i) bar_init(bars + 8 * i, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;\nfence.proxy.async.shared::cta;" ::: "memory");
+    }
+    __syncwarp();
+    const uint64_t once = policy_evict_first();  // a row's own pages are read once
+
+    const auto page_of = [&](int g) {
+        if (g >= groups) return 0;
+        const int pg = g < pre_groups ? a.prefix_table[g >> gpp] : own[(g - pre_groups) >> gpp];
+        if (pg >= 0 && pg < a.num_pages) return pg;
+        bad = true;
+        return a.num_pages;  // outside the pool: the load gives zeros
+    };
+    // K or V of group g into its half of a stage
+    const auto issue = [&](int g, int page, int stage, int is_v) {
+        if (g < groups && lane == 0) {
+            const int in_page = ((g < pre_groups ? g : g - pre_groups) * kGroup) & (a.page_size - 1);
+            const uint32_t bar = bars + 8 * (is_v * ST + stage), dst = base + (stage * 2 + is_v) * kTile;
+            bar_expect(bar, kTile);
 #pragma unroll
-            for (int i = 0; i < kGroup * CH / 32; ++i) {
-                const int t = (i * 32 + lane) / CH, c = (i * 32 + lane) % CH;
-                const bool live = ok && t < n;
-                const uint32_t off = t * HD * 2 + ((c ^ (t & 7)) << 4);
-                cp16(kd + off, ks + (live ? t * a.k_token_stride + c * 8 : 0), live);
-                cp16(vd + off, vs + (live ? t * a.v_token_stride + c * 8 : 0), live);
-            }
+            for (int h = 0; h < HD / 64; ++h)
+                tma_load4(dst + h * (kGroup * 128), is_v ? &vmap : &kmap, h * 64, kvh, in_page, page, bar, once);
         }
-        cp_commit();
     };
 
+    // K of a group is asked for as soon as the first product has used the K before it, V after the second
     int g_issue = g0, page = page_of(g0);
 #pragma unroll
     for (int s = 0; s < ST; ++s) {
         const int nextp = page_of(g_issue + step);
-        issue(g_issue, page, s);
+        issue(g_issue, page, s, 0);
+        issue(g_issue, page, s, 1);
         g_issue += step;
         page = nextp;
     }
@@ -246,35 +357,40 @@ __global__ void __launch_bounds__(kRowWarps * 32) k_prefix_rows(const PrefixPara
     }
 
     int stage = 0;
-    for (int g = g0; g < groups; g += step) {
-        cp_wait<ST - 1>();
-        __syncwarp();
+    uint32_t phase = 0;
+    bool lost = false, k_next = false;  // a wait ran out; the stage's next K has been asked for
+    int g = g0;
+    for (; g < groups; g += step) {
         const uint32_t kd = base + stage * 2 * kTile, vd = kd + kTile;
-        float s[NB][4];
+        if (!bar_wait_warp(bars + 8 * stage, phase, nullptr)) {
+            lost = true;
+            break;
+        }
+        float s[NB][4], s1[NB][4];  // two chains of products
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s[nb][i] = 0.f;
+            for (int i = 0; i < 4; ++i) s[nb][i] = s1[nb][i] = 0.f;
         {
             const int t = lane & 15;
-            const uint32_t row = kd + t * HD * 2;
+            const uint32_t row = kd + t * 128;
 #pragma unroll
             for (int k = 0; k < KS; ++k) {
                 uint32_t af[4];
-                ldsm4(af, row + (((2 * k + (lane >> 4)) ^ (t & 7)) << 4));
+                ldsm4(af, row + (k / 4) * (kGroup * 128) + (((2 * (k % 4) + (lane >> 4)) ^ (t & 7)) << 4));
 #pragma unroll
-                for (int nb = 0; nb < NB; ++nb) mma16816<T>(s[nb], af, qf[nb][k][0], qf[nb][k][1]);
+                for (int nb = 0; nb < NB; ++nb) mma16816<T>(k & 1 ? s1[nb] : s[nb], af, qf[nb][k][0], qf[nb][k][1]);
             }
         }
+        __syncwarp();
+        issue(g_issue, page, stage, 0);
         const int n = (g < pre_groups ? a.prefix_len - g * kGroup : len - (g - pre_groups) * kGroup);
         const bool lo = (lane >> 2) < n, hi = (lane >> 2) + 8 < n;
         bool raise = false;
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
-            s[nb][0] = lo ? s[nb][0] * p.scale_log2 : -INFINITY;
-            s[nb][1] = lo ? s[nb][1] * p.scale_log2 : -INFINITY;
-            s[nb][2] = hi ? s[nb][2] * p.scale_log2 : -INFINITY;
-            s[nb][3] = hi ? s[nb][3] * p.scale_log2 : -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[nb][i] = (i < 2 ? lo : hi) ? (s[nb][i] + s1[nb][i]) * p.scale_log2 : -INFINITY;
             raise |= fmaxf(s[nb][0], s[nb][2]) > m[nb][0] + kSlack || fmaxf(s[nb][1], s[nb][3]) > m[nb][1] + kSlack;
         }
         if (__any_sync(~0u, raise)) {
@@ -307,26 +423,51 @@ __global__ void __launch_bounds__(kRowWarps * 32) k_prefix_rows(const PrefixPara
             pb[nb][0] = movm_t(pack2<T>(p0, p1));
             pb[nb][1] = movm_t(pack2<T>(p2, p3));
         }
+        if (!bar_wait_warp(bars + 8 * (ST + stage), phase, nullptr)) {
+            lost = true;
+            k_next = g_issue < groups;
+            break;
+        }
+        if (n < kGroup) {
+            // what lies behind the last token may be NaN, and 0 * NaN is not 0
+            for (int x = n * 8 + lane; x < kGroup * 8; x += 32)
+#pragma unroll
+                for (int h = 0; h < HD / 64; ++h)
+                    *reinterpret_cast<uint4*>(sm + (vd - smem_addr(sm)) + h * (kGroup * 128) + x * 16) = make_uint4(0, 0, 0, 0);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+        }
         {
             const int t = (lane & 7) + ((lane >> 4) << 3);
-            const uint32_t row = vd + t * HD * 2;
+            const uint32_t row = vd + t * 128;
 #pragma unroll
             for (int k = 0; k < KS; ++k) {
                 uint32_t af[4];
-                ldsm4_t(af, row + (((2 * k + ((lane >> 3) & 1)) ^ (t & 7)) << 4));
+                ldsm4_t(af, row + (k / 4) * (kGroup * 128) + (((2 * (k % 4) + ((lane >> 3) & 1)) ^ (t & 7)) << 4));
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb) mma16816<T>(o[nb][k], af, pb[nb][0], pb[nb][1]);
             }
         }
         __syncwarp();
         const int nextp = page_of(g_issue + step);
-        issue(g_issue, page, stage);
+        issue(g_issue, page, stage, 1);
         g_issue += step;
         page = nextp;
-        stage = stage + 1 == ST ? 0 : stage + 1;
+        if (++stage == ST) {
+            stage = 0;
+            phase ^= 1;
+        }
     }
-    cp_wait<0>();
-    __syncwarp();
+    if (lost) {
+        // the result is lost; no copy may be in flight when the stages are used again: the oldest is at `stage`
+        bad = true;
+        for (int i = 0; i < 2 * ST; ++i) {
+            const int st = (stage + i / 2) % ST;
+            if (g + (i / 2) * step < groups) bar_wait_slow(bars + 8 * ((i & 1) * ST + st), phase ^ (st < stage), nullptr);
+        }
+        if (k_next) bar_wait_slow(bars + 8 * stage, phase ^ 1, nullptr);
+        __syncwarp();
+    }
 
     // this warp's partial to its part of shared memory: O [8*NB][HD], then (m, l) [8*NB]
     float* wo = reinterpret_cast<float*>(sm + warp * kWarp);
@@ -346,42 +487,25 @@ __global__ void __launch_bounds__(kRowWarps * 32) k_prefix_rows(const PrefixPara
             for (int i = 0; i < 4; ++i)
                 wo[(h + (i & 1)) * HD + k * 16 + (lane >> 2) + ((i >> 1) << 3)] = o[nb][k][i];
     }
-    if (C > 1) cluster_sync();
-    else __syncthreads();
-    pdl_wait();  // the prefix pass's partials
+    __syncthreads();
 
-    // the join: each CTA of the cluster takes its share of the outputs, four channels a thread
-    const uint32_t local = smem_addr(sm);
-    const int quads = heads * (HD / 4);
-    for (int x = rank * blockDim.x + threadIdx.x; x < quads; x += C * blockDim.x) {
-        const int h = x / (HD / 4), c = (x % (HD / 4)) * 4;
-        Join jn;
-        for (uint32_t k = 0; k < C; ++k) {
-            const uint32_t at = C > 1 ? map_rank(local, k) : local;
-            for (int w = 0; w < kRowWarps; ++w) {
-                const uint32_t wb = at + w * kWarp;
-                jn.add(ld_cluster2(wb + 8 * NB * HD * 4 + h * 8), ld_cluster4(wb + (h * HD + c) * 4));
-            }
-        }
-        if (!p.walk_prefix && a.prefix_len > 0) {
-            const int row = r * p.group + h0 + h, tile = row / p.tile_rows, in = row % p.tile_rows;
-            const long long u = (long long)kvh * p.row_tiles + tile;
-            const long long c0 = u * p.kv_tiles / p.per, c1 = ((u + 1) * p.kv_tiles - 1) / p.per;
-            const bool pair = p.tile_rows == 256;
-            const long long first = 2 * (c0 + u) + (pair ? in >> 7 : 0), past = 2 * (c1 + u) + 2;
-#pragma unroll 4
-            for (long long s = first; s < past; s += pair ? 2 : 1) {
-                const long long at = s * 128 + (in & 127);
-                jn.add(p.part_ml[at], *reinterpret_cast<const float4*>(p.part_o + at * HD + c));
-            }
-        }
-        const float inv = jn.L == 0.f ? 0.f : 1.f / jn.L;
-        T res[4] = {from_f32<T>(jn.o.x * inv), from_f32<T>(jn.o.y * inv), from_f32<T>(jn.o.z * inv), from_f32<T>(jn.o.w * inv)};
-        T* out = static_cast<T*>(a.out) + r * a.out_row_stride + (long long)(kvh * p.group + h0 + h) * a.out_head_stride + c;
+    // the join of the warps, a warp a query head
+    for (int h = warp; h < heads; h += kRowWarps) {
+        const int head = kvh * p.group + h0 + h;
+        const auto warp_o = [&](int w) { return reinterpret_cast<const float*>(sm + w * kWarp); };
+        float M, L, acc[HD / 32];
+        join_partials<HD>(kRowWarps, [&](int w) { return reinterpret_cast<const float2*>(warp_o(w) + 8 * NB * HD)[h]; },
+                          [&](int w) { return warp_o(w) + h * HD; }, M, L, acc);
+        if (p.join) {
+            const long long at = ((long long)split * a.num_rows + r) * a.num_q_heads + head;
+            if (lane == 0) p.own_ml[at] = make_float2(M, L);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) out[i] = res[i];
+            for (int c = 0; c < HD / 32; ++c) p.own_o[at * HD + lane * (HD / 32) + c] = acc[c];
+        } else {
+            store_out<T, HD>(p, L, acc, r, head);
+        }
     }
-    if (C > 1) cluster_sync();  // the others may still read this CTA's shared memory
+    if (last) pdl_wait();
 }
 
 }  // namespace tt

@@ -12,76 +12,36 @@
 // rescaled, only when a logit exceeds it by kSlack, as in the rows' pass.
 //
 // Work: units of (kv head, row tile), each kv_tiles key tiles; the flattened list is cut into equal spans,
-// one per CTA, so that every SM has the same number of tiles whatever the shape.  A span inside a unit
-// leaves one partial (m, l, O) per accumulator in the workspace, in slot 2 (cta + unit) + t, which no other
-// span has; the rows' pass joins them.
+// one per CTA, so that every SM has the same number of tiles whatever the shape.  Where the row tiles of a
+// kv head fill the SMs in whole groups, a group of CTAs takes the same span for all of them, so that each K
+// and V page comes from HBM once and from L2 for the rest of the group.  A span inside a unit leaves one
+// partial (m, l, O) per accumulator in the workspace, in a slot that no other span has; the join adds them.
 //
 // Warps: 0 loads K and V (TMA, one box per page and 64 channels, 128-byte swizzle), 1 issues the matrix
 // instructions, 2 clears the V rows behind the prefix's end (what lies there may be NaN, and 0 * NaN is not
 // 0), 4-7 and 8-11 are the softmax of the two accumulators and load their queries.
 #pragma once
-#include <cuda.h>
-
 #include "tt_prefix_rows.cuh"
 
 namespace tt {
 
-__device__ int g_prefix_error = 0;  // a bounded wait that ran out (TT_ERR_TIMEOUT); reported by tt_device_error
-
 constexpr int kPsThreads = 384;
 constexpr int kPsTile = 128;                       // keys per tile, rows per accumulator
-constexpr long long kPsPatience = 4000000000LL;    // clocks a wait may take (about two seconds)
 
 template <int HD, bool PAIR> struct PsShape {
     static constexpr int kSlot = kPsTile * HD * 2;                 // a K or V tile
     static constexpr int kHalf = kPsTile * 64 * 2;                 // 64 of its channels: 128-byte rows
     static constexpr int kQ = (PAIR ? 2 : 1) * kSlot;
-    static constexpr int kSlots = HD == 128 ? (PAIR ? 5 : 6) : 8;
-    static constexpr int kSmem = 1024 + kQ + kSlots * kSlot + 256; // alignment, tiles, barriers
+    static constexpr int kSlots = HD == 128 ? (PAIR ? 3 : 4) : 8;  // 160 KB with Q: leaves room for a CTA of the rows' pass
+    static constexpr int kSmem = kQ + kSlots * kSlot + 256;        // tiles, barriers
     static constexpr uint32_t kTmemO = 256;                        // S_0 S_1 in columns 0, 128; O_t behind
 };
 
 struct PsBars {  // in shared memory
-    uint64_t full[8], empty[8], q_full, s_full[2], p_ready[2], v_cut, v_fixed, drain;
+    uint64_t full[8], empty[8], q_full, s_full[2], p_ready[4], v_cut, v_fixed, drain;
     uint32_t tmem;
     int abort, bad;
 };
-
-__device__ __forceinline__ void bar_init(uint32_t b, uint32_t n) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(b), "r"(n) : "memory"); }
-__device__ __forceinline__ void bar_arrive(uint32_t b) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(b) : "memory"); }
-__device__ __forceinline__ void bar_expect(uint32_t b, uint32_t bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(b), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ bool bar_try(uint32_t b, uint32_t parity) {
-    uint32_t ok;
-    asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}"
-                 : "=r"(ok) : "r"(b), "r"(parity) : "memory");
-    return ok != 0;
-}
-// Bounded: false when it took too long here (recorded) or elsewhere in the CTA.
-__device__ __noinline__ bool bar_wait_slow(uint32_t b, uint32_t parity, volatile int* abort) {
-    const long long t0 = clock64();
-    while (clock64() - t0 < kPsPatience) {
-        if (bar_try(b, parity)) return true;
-        if (abort && *abort) return false;
-    }
-    if (abort) *abort = 1;
-    atomicCAS(&g_prefix_error, 0, (int)TT_ERR_TIMEOUT);
-    return false;
-}
-__device__ __forceinline__ bool bar_wait(uint32_t b, uint32_t parity, volatile int* abort) {
-    return bar_try(b, parity) || bar_wait_slow(b, parity, abort);
-}
-
-// The same by a whole warp, with one answer.
-__device__ __forceinline__ bool bar_wait_warp(uint32_t b, uint32_t parity, volatile int* abort) {
-    return __all_sync(~0u, bar_wait(b, parity, abort));
-}
-
-__device__ __forceinline__ void tma_load4(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, int c3, uint32_t bar) {
-    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
-                 ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar) : "memory");
-}
 
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -118,6 +78,21 @@ __device__ __forceinline__ void tc_st16(uint32_t addr, const uint32_t* v) {
 __device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// Two float32 at a time, as the FMA pipe takes them; the larger of three.
+__device__ __forceinline__ void fma2(float& x, float& y, float a, float b) {  // x = x a + b, y = y a + b
+    asm("{\n.reg .b64 v, a, b;\nmov.b64 v, {%0, %1};\nmov.b64 a, {%2, %2};\nmov.b64 b, {%3, %3};\n"
+        "fma.rn.f32x2 v, v, a, b;\nmov.b64 {%0, %1}, v;\n}" : "+f"(x), "+f"(y) : "f"(a), "f"(b));
+}
+__device__ __forceinline__ void add2(float& x, float& y, float a, float b) {  // x += a, y += b
+    asm("{\n.reg .b64 v, a;\nmov.b64 v, {%0, %1};\nmov.b64 a, {%2, %3};\nadd.rn.f32x2 v, v, a;\nmov.b64 {%0, %1}, v;\n}"
+        : "+f"(x), "+f"(y) : "f"(a), "f"(b));
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
 // Shared-memory operand descriptors, 128-byte swizzle.  K-major (rows of 64 channels, groups of eight rows
 // 1024 bytes apart) and MN-major (V: a token's 64 channels contiguous; groups of eight tokens 1024 bytes
 // apart, the next 64 channels `lbo` bytes on).
@@ -129,27 +104,28 @@ template <typename T> constexpr uint32_t ps_idesc(int n, bool b_mn) {
     return 1u << 4 | fmt << 7 | fmt << 10 | (b_mn ? 1u << 16 : 0u) | (uint32_t)(n >> 3) << 17 | (uint32_t)(kPsTile >> 4) << 24;
 }
 
-// The spans of this CTA: fn(unit, first key tile, key tiles) for each, until fn returns false.
+// The spans of this CTA: fn(kv head, row tile, slot, first key tile, key tiles) for each, until fn returns false.
 template <typename F>
 __device__ __forceinline__ void ps_spans(const PrefixParams& p, F fn) {
-    const long long total = (long long)p.a.num_kv_heads * p.row_tiles * p.kv_tiles;
-    long long f = (long long)blockIdx.x * p.per;
+    const long long total = (long long)p.units * p.kv_tiles;
+    const int group = blockIdx.x / p.lanes, lane = blockIdx.x % p.lanes;
+    long long f = (long long)group * p.per;
     const long long end = f + p.per < total ? f + p.per : total;
     while (f < end) {
         const int u = (int)(f / p.kv_tiles), k0 = (int)(f % p.kv_tiles);
         const int n = (int)(end - f < p.kv_tiles - k0 ? end - f : p.kv_tiles - k0);
-        if (!fn(u, k0, n)) return;
+        const int kvh = p.lanes > 1 ? u : u / p.row_tiles, tile = p.lanes > 1 ? lane : u % p.row_tiles;
+        if (!fn(kvh, tile, (long long)(group + u) * p.lanes + lane, k0, n)) return;
         f += n;
     }
 }
 
 template <typename T, int HD, bool PAIR>
-__global__ void __launch_bounds__(kPsThreads, 1)
+__global__ void __launch_bounds__(512, 1)  // 128 registers a thread, not the 168 that 384 threads could have
 k_prefix_shared(const PrefixParams p, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
     using S = PsShape<HD, PAIR>;
     constexpr int kLook = PAIR ? 1 : 2;  // key tiles whose first product is issued ahead
-    extern __shared__ unsigned char raw[];
-    unsigned char* sm = reinterpret_cast<unsigned char*>(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
+    extern __shared__ __align__(1024) unsigned char sm[];
     PsBars* bars = reinterpret_cast<PsBars*>(sm + S::kQ + S::kSlots * S::kSlot);
     const uint32_t q_s = smem_addr(sm), ring = q_s + S::kQ;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -167,7 +143,8 @@ k_prefix_shared(const PrefixParams p, const __grid_constant__ CUtensorMap kmap, 
         bar_init(q_full, PAIR ? 256 : 128);
         for (int t = 0; t < 2; ++t) {
             bar_init(s_full + 8 * t, 1);
-            bar_init(p_ready + 8 * t, 128);
+            bar_init(p_ready + 16 * t, 128);
+            bar_init(p_ready + 16 * t + 8, 128);
         }
         bar_init(v_cut, 1);
         bar_init(v_fixed, 32);
@@ -191,11 +168,11 @@ k_prefix_shared(const PrefixParams p, const __grid_constant__ CUtensorMap kmap, 
         // ---- K and V tiles into the ring, in the order the products take them
         const int box = a.page_size < kPsTile ? a.page_size : kPsTile;  // tokens per load
         const int boxes = kPsTile / box;
+        const uint64_t again = policy_evict_last();  // the other row tiles read it too
         uint32_t it = 0;
-        ps_spans(p, [&](int u, int k0, int n) {
-            const int kvh = u / p.row_tiles;
-            const auto load = [&](const CUtensorMap* map, int tile) {
-                const int t0 = (k0 + tile) * kPsTile;
+        ps_spans(p, [&](int kvh, int tile, long long slot_at, int k0, int n) {
+            const auto load = [&](const CUtensorMap* map, int kt) {
+                const int t0 = (k0 + kt) * kPsTile;
                 const int left = a.prefix_len - t0, use = left < kPsTile ? (left + box - 1) / box : boxes;
                 int page = a.num_pages;  // outside the pool: the load gives zeros
                 if (lane < use) {
@@ -213,7 +190,7 @@ k_prefix_shared(const PrefixParams p, const __grid_constant__ CUtensorMap kmap, 
                     const uint32_t dst = ring + slot * S::kSlot + lane * box * 128;
                     const int row = (t0 + lane * box) & (a.page_size - 1);
 #pragma unroll
-                    for (int h = 0; h < HD / 64; ++h) tma_load4(dst + h * S::kHalf, map, h * 64, kvh, row, page, full + 8 * slot);
+                    for (int h = 0; h < HD / 64; ++h) tma_load4(dst + h * S::kHalf, map, h * 64, kvh, row, page, full + 8 * slot, again);
                 }
                 ++it;
                 return true;
@@ -244,14 +221,16 @@ k_prefix_shared(const PrefixParams p, const __grid_constant__ CUtensorMap kmap, 
                     tc_mma_ss(tmem + t * 128, smem_desc(q + off, 16, 1024), smem_desc(k + off, 16, 1024), id_qk, s > 0);
                 }
             };
-            const auto pv = [&](int t, uint32_t i, bool acc) {
+            const auto pv = [&](int t, uint32_t i, int half, bool acc) {  // 64 of the tile's keys
                 const uint32_t v = slot_of(i);
 #pragma unroll
-                for (int s = 0; s < kPsTile / 16; ++s)
+                for (int k = 0; k < kPsTile / 32; ++k) {
+                    const int s = half * (kPsTile / 32) + k;
                     tc_mma_ts(tmem + S::kTmemO + t * HD, tmem + t * 128 + s * 8, smem_desc(v + s * 2048, S::kHalf, 1024), id_pv,
-                              acc || s > 0);
+                              acc || k > 0);
+                }
             };
-            ps_spans(p, [&](int u, int k0, int n) {
+            ps_spans(p, [&](int kvh, int tile, long long slot_at, int k0, int n) {
                 if (!bar_wait(q_full, q_phase, abort)) return false;
                 q_phase ^= 1;
                 tc_fence_after();
@@ -277,10 +256,13 @@ k_prefix_shared(const PrefixParams p, const __grid_constant__ CUtensorMap kmap, 
                         fix_phase ^= 1;
                     }
                     for (int t = PAIR ? 0 : j & 1; t < (PAIR ? 2 : (j & 1) + 1); ++t) {
-                        if (!bar_wait(p_ready + 8 * t, p_phase[t], abort)) return false;
+                        if (!bar_wait(p_ready + 16 * t, p_phase[t], abort)) return false;
+                        tc_fence_after();
+                        pv(t, vi, 0, PAIR ? j > 0 : j > 1);
+                        if (!bar_wait(p_ready + 16 * t + 8, p_phase[t], abort)) return false;
                         p_phase[t] ^= 1;
                         tc_fence_after();
-                        pv(t, vi, PAIR ? j > 0 : j > 1);
+                        pv(t, vi, 1, true);
                         if (!PAIR || t == 1) tc_commit(empty + 8 * (vi % S::kSlots));
                         if (more) {
                             if ((!PAIR || t == 0) && !slot_full(ki)) return false;
@@ -302,7 +284,7 @@ k_prefix_shared(const PrefixParams p, const __grid_constant__ CUtensorMap kmap, 
         // ---- V rows behind the end of the prefix
         if (a.prefix_len % kPsTile) {
             uint32_t loads = 0, phase = 0;
-            ps_spans(p, [&](int u, int k0, int n) {
+            ps_spans(p, [&](int kvh, int tile, long long slot_at, int k0, int n) {
                 loads += 2 * n;
                 if (k0 + n != p.kv_tiles) return true;
                 if (!bar_wait_warp(v_cut, phase, abort)) return false;
@@ -324,9 +306,9 @@ k_prefix_shared(const PrefixParams p, const __grid_constant__ CUtensorMap kmap, 
         const int rows_all = a.num_rows * p.group;
         const bool q16 = !(((uintptr_t)a.q & 15) | ((a.q_row_stride | a.q_head_stride) & 7));
         uint32_t phase = 0;
-        ps_spans(p, [&](int u, int k0, int n) {
-            const int kvh = u / p.row_tiles, mine = PAIR ? n : (n - t + 1) / 2;
-            const int mrow = (u % p.row_tiles) * p.tile_rows + (PAIR ? t * kPsTile : 0) + row;
+        ps_spans(p, [&](int kvh, int tile, long long slot_at, int k0, int n) {
+            const int mine = PAIR ? n : (n - t + 1) / 2;
+            const int mrow = tile * p.tile_rows + (PAIR ? t * kPsTile : 0) + row;
             const bool warp_on = mrow - lane < rows_all;  // any row of this warp
             if (PAIR || t == 0) {
                 // this row's query into the swizzled layout of the first product
@@ -353,60 +335,83 @@ k_prefix_shared(const PrefixParams p, const __grid_constant__ CUtensorMap kmap, 
                 if (!bar_wait_warp(s_full + 8 * t, phase, abort)) return false;
                 phase ^= 1;
                 tc_fence_after();
-                if (warp_on) {
-                    float s[kPsTile];
-                    uint32_t* su = reinterpret_cast<uint32_t*>(s);
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) tc_ld32(su + 32 * c, s_col + 32 * c);
+                // The upper half of S goes through the registers for its maximum only; the lower half stays in them,
+                // becomes weights first (its P lies over S columns that have been read) and the upper half is read
+                // again: 64 registers of S instead of 128, and the second product starts on the lower half.
+                float s[64];
+                uint32_t* su = reinterpret_cast<uint32_t*>(s);
+                const int left = a.prefix_len - (k0 + (PAIR ? i : 2 * i + t)) * kPsTile;
+                const auto get = [&](int from) {
+                    tc_ld32(su, s_col + from);
+                    tc_ld32(su + 32, s_col + from + 32);
                     tc_wait_ld();
-                    const int left = a.prefix_len - (k0 + (PAIR ? i : 2 * i + t)) * kPsTile;
                     if (left < kPsTile) {
 #pragma unroll
-                        for (int c = 0; c < kPsTile; ++c) s[c] = c < left ? s[c] : -INFINITY;
+                        for (int c = 0; c < 64; ++c) s[c] = from + c < left ? s[c] : -INFINITY;
                     }
+                };
+                float lsum[2] = {0.f, 0.f};
+                float neg = 0.f;
+                const auto put = [&](int from) {  // weights of the 64 columns in s
+#pragma unroll
+                    for (int c = 0; c < 64; c += 32) {
+                        uint32_t w[16];
+#pragma unroll
+                        for (int k = 0; k < 16; ++k) {
+                            float x = s[c + 2 * k], y = s[c + 2 * k + 1];
+                            fma2(x, y, p.scale_log2, neg);
+                            x = fast_exp2(x);
+                            y = fast_exp2(y);
+                            add2(lsum[0], lsum[1], x, y);
+                            w[k] = pack2<T>(x, y);
+                        }
+                        tc_st16(s_col + (from + c) / 2, w);
+                    }
+                };
+                if (warp_on) {
+                    get(64);
                     float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-                    for (int c = 4; c < kPsTile; ++c) mx[c & 3] = fmaxf(mx[c & 3], s[c]);
-                    const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
+                    for (int c = 4; c < 64; c += 2) mx[c / 2 & 3] = max3(mx[c / 2 & 3], s[c], s[c + 1]);
+                    get(0);
+#pragma unroll
+                    for (int c = 0; c < 64; c += 2) mx[c / 2 & 3] = max3(mx[c / 2 & 3], s[c], s[c + 1]);
+                    const float top = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * p.scale_log2;
                     if (__any_sync(~0u, top > m + kSlack)) {
                         const float nm = fmaxf(m, top);
                         const float f = nm == m ? 1.f : m == -INFINITY ? 0.f : fast_exp2(m - nm);
                         m = nm;
                         l *= f;
-                        if (i > 0) {
-#pragma unroll
+                        if (i > 0) {  // the arrival on s_full says that O has every step before this one
+#pragma unroll 1
                             for (int c = 0; c < HD / 32; ++c) {
-                                uint32_t o[32];
+                                uint32_t* o = su;  // S is read again afterwards
                                 tc_ld32(o, o_col + 32 * c);
                                 tc_wait_ld();
 #pragma unroll
                                 for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
                                 tc_st32(o_col + 32 * c, o);
                             }
+                            get(0);
                         }
                     }
-                    const float me = m == -INFINITY ? 0.f : m;
-                    float ls[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        uint32_t w[16];
-#pragma unroll
-                        for (int k = 0; k < 16; ++k) {
-                            const float x = fast_exp2(fmaf(s[32 * c + 2 * k], p.scale_log2, -me));
-                            const float y = fast_exp2(fmaf(s[32 * c + 2 * k + 1], p.scale_log2, -me));
-                            ls[k & 3] += x + y;
-                            w[k] = pack2<T>(x, y);
-                        }
-                        tc_st16(s_col + 16 * c, w);
-                    }
-                    l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
+                    neg = m == -INFINITY ? 0.f : -m;
+                    put(0);
                     tc_wait_st();
                 }
                 tc_fence_before();
-                bar_arrive(p_ready + 8 * t);
+                bar_arrive(p_ready + 16 * t);
+                if (warp_on) {
+                    get(64);
+                    put(64);
+                    l += lsum[0] + lsum[1];
+                    tc_wait_st();
+                }
+                tc_fence_before();
+                bar_arrive(p_ready + 16 * t + 8);
             }
             // the span's partial
-            const long long slot = 2LL * (blockIdx.x + u) + t;
+            const long long slot = 2 * slot_at + t;
             if (mine > 0) {
                 if (!bar_wait_warp(s_full + 8 * t, phase, abort)) return false;
                 phase ^= 1;
@@ -432,8 +437,8 @@ k_prefix_shared(const PrefixParams p, const __grid_constant__ CUtensorMap kmap, 
         });
         if (*abort) {
             // a wait ran out: nothing that this CTA was to leave may be taken for a result
-            ps_spans(p, [&](int u, int k0, int n) {
-                p.part_ml[(2LL * (blockIdx.x + u) + t) * kPsTile + row] = make_float2(-INFINITY, NAN);
+            ps_spans(p, [&](int kvh, int tile, long long slot_at, int k0, int n) {
+                p.part_ml[(2 * slot_at + t) * kPsTile + row] = make_float2(-INFINITY, NAN);
                 return true;
             });
         }

@@ -258,7 +258,8 @@ def shared_prefix_attention(q, k_pages, v_pages, prefix_table, prefix_len, table
     scale = hd ** -0.5 if scale is None else float(scale)
     if not math.isfinite(scale):
         raise ValueError("scale must be finite.")
-    ks, vs = k_pages.stride(), v_pages.stride()
+    # the stride of a dimension of one entry says nothing
+    ks, vs = (tuple(st if n > 1 else hd for n, st in zip(t.shape, t.stride())) for t in (k_pages, v_pages))
     rest = (q.stride(0), q.stride(1), out.stride(0), out.stride(1), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], tables.stride(0),
             R, nq, nkv, hd, P, k_pages.shape[0], prefix_len, W, B, _DT[dt], scale, 0)
     L = lib()
