@@ -9,6 +9,7 @@ namespace tt {
 static_assert(sizeof(tt_shared_prefix_args) == 208, "packed by paged.py");
 
 constexpr int kSms = 148;
+constexpr int kCross = 4;  // measured: 7 tiles in 30 us, 7 in two spans in 40 (384 rows of heads on 8k)
 
 // All kernels ask for the whole of an SM's shared memory: the passes' CTAs share one, and an SM that has to
 // divide its memory anew between two kernels has to run dry first.
@@ -94,7 +95,9 @@ static tt_status check_prefix(const tt_shared_prefix_args* args) {
     return TT_OK;
 }
 
-static int prefix_groups(const PrefixParams& p) { return (int)(((long long)p.units * p.kv_tiles + p.per - 1) / p.per); }
+static int prefix_groups(const PrefixParams& p) {
+    return p.spans ? p.units * p.spans : (int)(((long long)p.units * p.kv_tiles + p.per - 1) / p.per);
+}
 static size_t prefix_slots(const PrefixParams& p) {
     return p.walk_prefix ? 0 : 2 * ((size_t)prefix_groups(p) + (size_t)p.units) * p.lanes;
 }
@@ -118,10 +121,18 @@ static PrefixParams plan_prefix(const tt_shared_prefix_args& a) {
         // CTA groups over all row tiles of a kv head, unless they would leave more than a tenth of the SMs idle
         p.lanes = kSms / p.row_tiles * p.row_tiles * 10 >= kSms * 9 ? p.row_tiles : 1;
         p.units = a.num_kv_heads * (p.row_tiles / p.lanes);
-        const long long total = (long long)p.units * p.kv_tiles, groups = kSms / p.lanes;
-        p.per = (int)((total + groups - 1) / groups);
-        // one 128-row tile: a span of one key tile would leave its second accumulator without work
-        if (p.tile_rows == kPsTile && p.per < 2) p.per = 2;
+        const int groups = kSms / p.lanes;
+        // Equal spans across units use every SM, but a CTA whose span crosses a unit's border starts and ends twice,
+        // which costs it about kCross key tiles; whole spans per unit may leave SMs idle.
+        p.per = (int)(((long long)p.units * p.kv_tiles + groups - 1) / groups);
+        if (p.units <= groups) {
+            const int whole = (p.kv_tiles + groups / p.units - 1) / (groups / p.units);
+            if (whole <= p.per + kCross) p.per = whole, p.spans = 1;
+        }
+        // A span of one key tile leaves as many bytes of partials as two, and a 128-row tile's second accumulator
+        // without work (64 rows of 32 heads on 2k: 27.8 -> 23.2 us; at least four tiles: 25.5).
+        if (p.per < 2) p.per = 2;
+        if (p.spans) p.spans = (p.kv_tiles + p.per - 1) / p.per;
     }
     // CTAs of the rows' pass per row and head tile: two for each SM in all, if that leaves a warp two groups
     const long long tokens = (long long)a.table_width * a.page_size + (p.walk_prefix ? a.prefix_len : 0);

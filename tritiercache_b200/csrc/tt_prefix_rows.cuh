@@ -42,12 +42,12 @@ struct PrefixParams {
     int head_tiles;              // tiles of 8*NB query heads per kv head
     int splits;                  // CTAs per row and head tile in the rows' pass
     // prefix pass: a unit is a kv head and one tile of tile_rows rows of its (row, head of the group) matrix, or
-    // with lanes = row_tiles all its tiles at once, one CTA of a group of `lanes` each; the flattened (unit, key
-    // tile) list is cut into spans of `per`, one per CTA group.  A span's partials are in slots
-    // 2 ((group + unit) lanes + lane) + t of 128 rows: t is the half of a 256-row tile, or even and odd key tiles
-    // of a 128-row one
+    // with lanes = row_tiles all its tiles at once, one CTA of a group of `lanes` each.  The flattened (unit, key
+    // tile) list is cut into spans of `per` for the groups: `spans` a unit, or, with spans = 0, across units.
+    // A span's partials are in slots 2 ((group + unit) lanes + lane) + t of 128 rows: t is the half of a 256-row
+    // tile, or even and odd key tiles of a 128-row one
     int walk_prefix;             // 1: no prefix pass, the rows' pass reads the prefix too
-    int tile_rows, row_tiles, lanes, units, kv_tiles, per;
+    int tile_rows, row_tiles, lanes, units, kv_tiles, per, spans;
     float* part_o;               // [slot][128][hd]
     float2* part_ml;             // [slot][128] (m in log2 units, l)
     int join;                    // 1: the rows' pass leaves partials [splits][num_rows][num_q_heads] for k_prefix_join; 0: outputs
@@ -220,7 +220,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32) k_prefix_join(const PrefixPar
         const int tile = row / p.tile_rows, in = row % p.tile_rows, lane = p.lanes > 1 ? tile : 0;
         const bool pair = p.tile_rows == 256;
         const int u = p.lanes > 1 ? kvh : kvh * p.row_tiles + tile;
-        const int g0 = u * p.kv_tiles / p.per, g1 = ((u + 1) * p.kv_tiles - 1) / p.per;
+        const int g0 = p.spans ? u * p.spans : u * p.kv_tiles / p.per;
+        const int g1 = p.spans ? g0 + p.spans - 1 : ((u + 1) * p.kv_tiles - 1) / p.per;
         // even and odd key tiles are neighbours (!pair has one row tile, so one lane)
         first = (2 * ((long long)(g0 + u) * p.lanes + lane) + (pair ? in >> 7 : 0)) * 128 + (in & 127);
         step = (pair ? 2 * p.lanes : 1) * 128;

@@ -11,8 +11,8 @@
 // and O_t += P_t V (P from tensor memory, V from shared memory).  m is a reference that is raised, and O
 // rescaled, only when a logit exceeds it by kSlack, as in the rows' pass.
 //
-// Work: units of (kv head, row tile), each kv_tiles key tiles; the flattened list is cut into equal spans,
-// one per CTA, so that every SM has the same number of tiles whatever the shape.  Where the row tiles of a
+// Work: units of (kv head, row tile), each kv_tiles key tiles; the flattened list is cut into spans, one per
+// CTA, so that every SM has about the same number of tiles whatever the shape.  Where the row tiles of a
 // kv head fill the SMs in whole groups, a group of CTAs takes the same span for all of them, so that each K
 // and V page comes from HBM once and from L2 for the rest of the group.  A span inside a unit leaves one
 // partial (m, l, O) per accumulator in the workspace, in a slot that no other span has; the join adds them.
@@ -78,6 +78,14 @@ __device__ __forceinline__ void tc_st16(uint32_t addr, const uint32_t* v) {
 __device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// One thread of the warp, known as such to the compiler: operands of the tcgen05 instructions it issues are
+// uniform.  (With `lane == 0` instead each product took about 70 clocks to issue.)
+__device__ __forceinline__ bool elect_one() {
+    uint32_t ok;
+    asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(ok));
+    return ok != 0;
+}
+
 // Two float32 at a time, as the FMA pipe takes them; the larger of three.
 __device__ __forceinline__ void fma2(float& x, float& y, float a, float b) {  // x = x a + b, y = y a + b
     asm("{\n.reg .b64 v, a, b;\nmov.b64 v, {%0, %1};\nmov.b64 a, {%2, %2};\nmov.b64 b, {%3, %3};\n"
@@ -105,15 +113,22 @@ template <typename T> constexpr uint32_t ps_idesc(int n, bool b_mn) {
 }
 
 // The spans of this CTA: fn(kv head, row tile, slot, first key tile, key tiles) for each, until fn returns false.
+// p.spans > 0: so many spans a unit, none crosses units; else the flattened list in spans of p.per.
 template <typename F>
 __device__ __forceinline__ void ps_spans(const PrefixParams& p, F fn) {
-    const long long total = (long long)p.units * p.kv_tiles;
     const int group = blockIdx.x / p.lanes, lane = blockIdx.x % p.lanes;
-    long long f = (long long)group * p.per;
-    const long long end = f + p.per < total ? f + p.per : total;
+    long long f, end;
+    if (p.spans) {
+        const long long u = group / p.spans;
+        f = u * p.kv_tiles + (long long)(group % p.spans) * p.per;
+        end = min(f + p.per, (u + 1) * p.kv_tiles);
+    } else {
+        f = (long long)group * p.per;
+        end = min(f + p.per, (long long)p.units * p.kv_tiles);
+    }
     while (f < end) {
         const int u = (int)(f / p.kv_tiles), k0 = (int)(f % p.kv_tiles);
-        const int n = (int)(end - f < p.kv_tiles - k0 ? end - f : p.kv_tiles - k0);
+        const int n = (int)min(end - f, (long long)(p.kv_tiles - k0));
         const int kvh = p.lanes > 1 ? u : u / p.row_tiles, tile = p.lanes > 1 ? lane : u % p.row_tiles;
         if (!fn(kvh, tile, (long long)(group + u) * p.lanes + lane, k0, n)) return;
         f += n;
@@ -208,26 +223,25 @@ k_prefix_shared(const PrefixParams p, const __grid_constant__ CUtensorMap kmap, 
                 bar_wait_slow(full + 8 * (i % S::kSlots), (i / S::kSlots) & 1, nullptr);
     } else if (warp == 1) {
         // ---- the matrix instructions, from one thread
-        if (lane == 0) {
+        if (elect_one()) {
             constexpr uint32_t id_qk = ps_idesc<T>(kPsTile, false), id_pv = ps_idesc<T>(HD, true);
             uint32_t it = 0, q_phase = 0, fix_phase = 0, p_phase[2] = {0, 0};
             const auto slot_of = [&](uint32_t i) { return ring + (i % S::kSlots) * S::kSlot; };
             const auto slot_full = [&](uint32_t i) { return bar_wait(full + 8 * (i % S::kSlots), (i / S::kSlots) & 1, abort); };
             const auto qk = [&](int t, uint32_t i) {
-                const uint32_t q = q_s + (PAIR ? t * S::kSlot : 0), k = slot_of(i);
+                const uint64_t q = smem_desc(q_s + (PAIR ? t * S::kSlot : 0), 16, 1024), k = smem_desc(slot_of(i), 16, 1024);
 #pragma unroll
                 for (int s = 0; s < HD / 16; ++s) {
-                    const uint32_t off = (s / 4) * S::kHalf + (s % 4) * 32;
-                    tc_mma_ss(tmem + t * 128, smem_desc(q + off, 16, 1024), smem_desc(k + off, 16, 1024), id_qk, s > 0);
+                    const int off = ((s / 4) * S::kHalf + (s % 4) * 32) / 16;  // addresses in units of 16 bytes
+                    tc_mma_ss(tmem + t * 128, q + off, k + off, id_qk, s > 0);
                 }
             };
             const auto pv = [&](int t, uint32_t i, int half, bool acc) {  // 64 of the tile's keys
-                const uint32_t v = slot_of(i);
+                const uint64_t v = smem_desc(slot_of(i), S::kHalf, 1024);
 #pragma unroll
                 for (int k = 0; k < kPsTile / 32; ++k) {
                     const int s = half * (kPsTile / 32) + k;
-                    tc_mma_ts(tmem + S::kTmemO + t * HD, tmem + t * 128 + s * 8, smem_desc(v + s * 2048, S::kHalf, 1024), id_pv,
-                              acc || k > 0);
+                    tc_mma_ts(tmem + S::kTmemO + t * HD, tmem + t * 128 + s * 8, v + s * 2048 / 16, id_pv, acc || k > 0);
                 }
             };
             ps_spans(p, [&](int kvh, int tile, long long slot_at, int k0, int n) {
