@@ -2,6 +2,8 @@
 // tt_shared_prefix_attention).
 #include <limits.h>
 
+#include <atomic>
+
 #include "tt_prefix_shared.cuh"
 
 namespace tt {
@@ -12,12 +14,18 @@ constexpr int kSms = 148;
 constexpr int kCross = 4;  // measured: 7 tiles in 30 us, 7 in two spans in 40 (384 rows of heads on 8k)
 
 // All kernels ask for the whole of an SM's shared memory: the passes' CTAs share one, and an SM that has to
-// divide its memory anew between two kernels has to run dry first.
-template <typename K>
-static cudaError_t set_smem(K* kern, size_t bytes) {
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-    if (e != cudaSuccess) return e;
-    return cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+// divide its memory anew between two kernels has to run dry first.  Once per kernel and device.
+template <auto Kern>
+static cudaError_t set_smem(size_t bytes) {
+    static std::atomic<unsigned long long> done{0};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    const unsigned long long bit = dev < 64 ? 1ull << dev : 0;
+    if (e != cudaSuccess || (done.load(std::memory_order_acquire) & bit)) return e;
+    e = cudaFuncSetAttribute(Kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(Kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+    return e;
 }
 
 template <typename T, int HD, int NB>
@@ -25,7 +33,7 @@ static cudaError_t launch_rows(const PrefixParams& p, const CUtensorMap& km, con
     constexpr int ST = HD == 64 ? 4 : 2;
     constexpr size_t smem = row_smem<HD, NB, ST>();
     auto* kern = k_prefix_rows<T, HD, NB, ST>;
-    const cudaError_t e = set_smem(kern, smem);
+    const cudaError_t e = set_smem<k_prefix_rows<T, HD, NB, ST>>(smem);
     if (e != cudaSuccess) return e;
     const dim3 grid((unsigned)(p.a.num_rows * p.splits), (unsigned)(p.a.num_kv_heads * p.head_tiles));
     return launch(kern, grid, dim3(kRowWarps * 32), smem, st, !p.walk_prefix, p, km, vm);
@@ -40,7 +48,7 @@ static cudaError_t launch_rows_t(const PrefixParams& p, const CUtensorMap& km, c
 
 template <typename T, int HD, int W>
 static cudaError_t launch_join_w(const PrefixParams& p, cudaStream_t st) {
-    const cudaError_t e = set_smem(k_prefix_join<T, HD, W>, 0);
+    const cudaError_t e = set_smem<k_prefix_join<T, HD, W>>(0);
     if (e != cudaSuccess) return e;
     const long long warps = (long long)p.a.num_rows * p.a.num_q_heads * W;
     return launch(k_prefix_join<T, HD, W>, dim3((unsigned)((warps + kJoinWarps - 1) / kJoinWarps)), dim3(kJoinWarps * 32), 0, st, true, p);
@@ -183,7 +191,7 @@ static cudaError_t launch_shared(const PrefixParams& p, const CUtensorMap& km, c
     using S = PsShape<HD, PAIR>;
     static_assert(sizeof(PsBars) <= 256 && S::kSmem <= 227 * 1024 && S::kSlots <= 8, "shared memory of the prefix pass");
     auto* kern = k_prefix_shared<T, HD, PAIR>;
-    const cudaError_t e = set_smem(kern, S::kSmem);
+    const cudaError_t e = set_smem<k_prefix_shared<T, HD, PAIR>>(S::kSmem);
     if (e != cudaSuccess) return e;
     return launch(kern, dim3((unsigned)(prefix_groups(p) * p.lanes)), dim3(kPsThreads), S::kSmem, st, false, p, km, vm);
 }

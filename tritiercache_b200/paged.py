@@ -11,54 +11,81 @@ impossible one does is said at each call.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import math
 import struct
-from typing import Optional
+import threading
 
 import torch
 
 from ._lib import check, lib
 
-_DT = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-_I32, _I64 = torch.int32, torch.int64
+_F32, _BF16, _F16, _I32, _I64 = torch.float32, torch.bfloat16, torch.float16, torch.int32, torch.int64
+_DT = {_F32: 0, _BF16: 1, _F16: 2}
 
 # the argument structs of the C ABI, packed with native alignment
 _TABLES = struct.Struct("@14Pq6i")
 _ROPE = struct.Struct("@12P18q12ifi")
 _PREFIX = struct.Struct("@9P11q10ifi")
 
-
-def _device(t, name: str):
-    if not isinstance(t, torch.Tensor) or not t.is_cuda:
-        raise ValueError(f"{name} must be a CUDA tensor (there is no CPU path).")
-    return t.device
-
-
-def _gaps(t) -> bool:
-    """Whether neighbours along the last dimension do not lie side by side."""
-    return t.shape[-1] > 1 and t.stride(-1) != 1 and t.numel() > 0
+# torch.cuda.current_stream() builds a Stream object, at half the price of a whole call here
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+    (lambda index: torch.cuda.current_stream(index).cuda_stream)
+_local = threading.local()
 
 
-def _vec(t, name: str, dev, dtype, n: Optional[int] = None):
-    """Address of a contiguous 1-D tensor of `dtype` with n elements (None: any)."""
-    if not isinstance(t, torch.Tensor) or t.device != dev:
-        raise ValueError(f"{name} must be a tensor on {dev}.")
-    if t.dtype != dtype or t.dim() != 1 or (n is not None and t.shape[0] != n) or not t.is_contiguous():
-        raise ValueError(f"{name} must be contiguous {dtype} of shape [{'n' if n is None else n}], got {t.dtype} "
-                         f"{tuple(t.shape)}.")
+def _vec(t, name: str, index: int, dtype, n: int) -> int:
+    """Address of a contiguous 1-D tensor of n elements."""
+    if t.dtype is not dtype or t.shape != (n,) or t.get_device() != index or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape [{n}] on cuda:{index}, got {t.dtype} "
+                         f"{tuple(t.shape)} on {t.device}.")
     return t.data_ptr()
 
 
-def _run(fn, packed: bytes, dev, what: str) -> None:
-    if torch.cuda.current_device() == dev.index:
-        st = fn(packed, torch.cuda.current_stream().cuda_stream)
+def _rows(t, name: str, index: int, dtype, shape):
+    """Strides of a tensor of this shape whose last dimension has no gaps."""
+    st = t.stride()
+    if t.dtype is not dtype or t.shape != shape or t.get_device() != index or \
+            (st[-1] != 1 and shape[-1] > 1 and t.numel() > 0):
+        raise ValueError(f"{name} must be {dtype} {tuple(shape)} on cuda:{index} without gaps in its last dimension, got {t.dtype} "
+                         f"{tuple(t.shape)}, strides {tuple(st)}, on {t.device}.")
+    return st
+
+
+def _apart(t, st, name: str) -> None:
+    """An output whose dimensions overlap (an expanded one) would be written by several threads."""
+    if 0 in st and any(d == 0 and n > 1 for n, d in zip(t.shape, st)):
+        raise ValueError(f"{name} is an output and must not be an expanded tensor.")
+
+
+def _device(t, name: str) -> int:
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor (there is no CPU path).")
+    return t.get_device()
+
+
+def _run(fn, packed: bytes, index: int, what: str) -> None:
+    if torch.cuda.current_device() == index:
+        st = fn(packed, _raw_stream(index))
     else:
-        with torch.cuda.device(dev):
-            st = fn(packed, torch.cuda.current_stream().cuda_stream)
+        with torch.cuda.device(index):
+            st = fn(packed, _raw_stream(index))
     if st:
         check(st, what)
 
 
+def _tensors_only(fn):
+    """What is not a tensor has none of a tensor's attributes."""
+    @functools.wraps(fn)
+    def call(*args, **kw):
+        try:
+            return fn(*args, **kw)
+        except AttributeError as e:
+            raise ValueError(f"{fn.__name__} takes tensors: {e}") from None
+    return call
+
+
+@_tensors_only
 def page_tables(ctx_lens, new_lens, tables, free_pages, free_count, page_size, seq_lens, cu_new, slots, positions,
                 row_seq, row_lens, deferred, free_count_out=None, position_offset=0) -> None:
     """Gives a step's new tokens their pages, slots and positions.
@@ -74,50 +101,31 @@ def page_tables(ctx_lens, new_lens, tables, free_pages, free_count, page_size, s
     position_offset), ``row_seq``, ``row_lens`` (-1, 0, -1, 0 for padding), and
     ``deferred`` [1], the number of deferred requests.  All int32 but slots.
     """
-    dev = _device(tables, "tables")
-    if tables.dtype != _I32 or tables.dim() != 2 or _gaps(tables):
-        raise ValueError("tables must be int32 [requests, width] with contiguous rows.")
+    index = _device(tables, "tables")
+    if tables.dim() != 2:
+        raise ValueError("tables must be int32 [requests, width].")
     B, W = tables.shape
-    n = slots.shape[0] if isinstance(slots, torch.Tensor) and slots.dim() == 1 else None
-    ps = [_vec(ctx_lens, "ctx_lens", dev, _I32, B), _vec(new_lens, "new_lens", dev, _I32, B), tables.data_ptr(),
-          _vec(free_pages, "free_pages", dev, _I32), _vec(free_count, "free_count", dev, _I32, 1),
-          _vec(free_count if free_count_out is None else free_count_out, "free_count_out", dev, _I32, 1),
-          _vec(seq_lens, "seq_lens", dev, _I32, B), _vec(cu_new, "cu_new", dev, _I32, B + 1),
-          _vec(slots, "slots", dev, _I64), _vec(positions, "positions", dev, _I32, n),
-          _vec(row_seq, "row_seq", dev, _I32, n), _vec(row_lens, "row_lens", dev, _I32, n),
-          _vec(deferred, "deferred", dev, _I32, 1)]
+    ts = _rows(tables, "tables", index, _I32, tables.shape)
+    if B > 1 and ts[0] < W:
+        raise ValueError("tables is written and its rows must not overlap.")
+    n = slots.numel()
+    cap = free_pages.numel()
+    fc = _vec(free_count, "free_count", index, _I32, 1)
     L = lib()
     size = L.tt_page_tables_workspace(B, n)
-    ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
-    _run(L.tt_page_tables, _TABLES.pack(*ps, 0 if ws is None else ws.data_ptr(), tables.stride(0) if B > 1 else max(W, 1), B, W,
-                                        free_pages.shape[0], int(page_size), n, int(position_offset)), dev, "page_tables")
+    ws = torch.empty(size, dtype=torch.uint8, device=tables.device) if size else None
+    packed = _TABLES.pack(_vec(ctx_lens, "ctx_lens", index, _I32, B), _vec(new_lens, "new_lens", index, _I32, B), tables.data_ptr(),
+                          _vec(free_pages, "free_pages", index, _I32, cap), fc,
+                          fc if free_count_out is None else _vec(free_count_out, "free_count_out", index, _I32, 1),
+                          _vec(seq_lens, "seq_lens", index, _I32, B), _vec(cu_new, "cu_new", index, _I32, B + 1),
+                          _vec(slots, "slots", index, _I64, n), _vec(positions, "positions", index, _I32, n),
+                          _vec(row_seq, "row_seq", index, _I32, n), _vec(row_lens, "row_lens", index, _I32, n),
+                          _vec(deferred, "deferred", index, _I32, 1), ws.data_ptr() if size else 0, ts[0] if B > 1 else W, B, W, cap,
+                          page_size, n, position_offset)
+    _run(L.tt_page_tables, packed, index, "page_tables")
 
 
-def _heads(t, name: str, dev, dtype, rows, heads, hd):
-    if not isinstance(t, torch.Tensor) or t.device != dev:
-        raise ValueError(f"{name} must be a tensor on {dev}.")
-    if t.dtype != dtype or t.shape != (rows, heads, hd) or _gaps(t):
-        raise ValueError(f"{name} must be {dtype} {(rows, heads, hd)} with contiguous channels, got {t.dtype} "
-                         f"{tuple(t.shape)}, strides {tuple(t.stride())}.")
-    return t.data_ptr()
-
-
-def _apart(t, name: str) -> None:
-    """An output whose dimensions overlap (an expanded one) would be written by several threads."""
-    for n, st in zip(t.shape, t.stride()):
-        if n > 1 and st == 0:
-            raise ValueError(f"{name} is an output and must not be an expanded tensor.")
-
-
-def _pool(t, name: str, dev, dtype, heads, hd):
-    if not isinstance(t, torch.Tensor) or t.device != dev:
-        raise ValueError(f"{name} must be a tensor on {dev}.")
-    if t.dtype != dtype or t.dim() != 4 or t.shape[2] != heads or t.shape[3] != hd or _gaps(t):
-        raise ValueError(f"{name} must be {dtype} [pages, page_size, {heads}, {hd}] with contiguous channels, got {t.dtype} "
-                         f"{tuple(t.shape)}, strides {tuple(t.stride())}.")
-    return t.data_ptr()
-
-
+@_tensors_only
 def qk_norm_rope(q, k, v, cos, sin, q_out, k_dst, v_dst, q_weight=None, k_weight=None, eps=1e-6, positions=None,
                  slots=None) -> None:
     """RMS norm of every query and key head (where its weight is given),
@@ -135,80 +143,70 @@ def qk_norm_rope(q, k, v, cos, sin, q_out, k_dst, v_dst, q_weight=None, k_weight
     every output; a position outside the tables makes the rotated channels NaN.
     q_out may be q itself, dense k_dst and v_dst k and v.
     """
-    dev = _device(q, "q")
+    index = _device(q, "q")
     dt = q.dtype
-    if dt not in _DT or q.dim() != 3:
-        raise ValueError("q must be float32, bfloat16 or float16 [rows, heads, head_dim].")
-    R, nq, hd = q.shape
-    if not isinstance(k, torch.Tensor) or k.dim() != 3:
-        raise ValueError("k must be a tensor [rows, kv_heads, head_dim].")
+    if dt not in _DT or q.dim() != 3 or k.dim() != 3:
+        raise ValueError("q and k must be float32, bfloat16 or float16 [rows, heads, head_dim].")
+    R, nq, hd = shape = q.shape
     nkv = k.shape[1]
-    for t, name in ((q_out, "q_out"), (k_dst, "k_dst")):
-        if not isinstance(t, torch.Tensor) or t.dtype not in (dt, torch.float32):
-            raise ValueError(f"{name} must be a tensor of {dt} or float32.")
-        _apart(t, name)
+    kv_shape = (R, nkv, hd)
+    qt, kt = q_out.dtype, k_dst.dtype
+    if (qt is not dt and qt is not _F32) or (kt is not dt and kt is not _F32):
+        raise ValueError(f"q_out, k_dst and v_dst must be {dt} or float32.")
     if (v is None) != (v_dst is None):
         raise ValueError("v and v_dst come together.")
-    if v_dst is not None:
-        if not isinstance(v_dst, torch.Tensor):
-            raise ValueError("v_dst must be a tensor.")
-        _apart(v_dst, "v_dst")
-    kt = k_dst.dtype
-    pq, pk, po = _heads(q, "q", dev, dt, R, nq, hd), _heads(k, "k", dev, dt, R, nkv, hd), _heads(q_out, "q_out", dev, q_out.dtype, R, nq, hd)
-    pv = 0 if v is None else _heads(v, "v", dev, dt, R, nkv, hd)
+    qs, os = _rows(q, "q", index, dt, shape), _rows(q_out, "q_out", index, qt, shape)
+    ks = _rows(k, "k", index, dt, kv_shape)
     if slots is None:
-        pkd = _heads(k_dst, "k_dst", dev, kt, R, nkv, hd)
-        pvd = 0 if v is None else _heads(v_dst, "v_dst", dev, kt, R, nkv, hd)
-        psl, pages, psize = 0, R, 1
-        kst = (k_dst.stride(0), 0, k_dst.stride(1))
-        vst = (0, 0, 0) if v is None else (v_dst.stride(0), 0, v_dst.stride(1))
+        dst, psl, pages, psize = kv_shape, 0, R, 1
     else:
-        pkd = _pool(k_dst, "k_dst", dev, kt, nkv, hd)
-        pvd = 0
-        if v is not None:
-            pvd = _pool(v_dst, "v_dst", dev, kt, nkv, hd)
-            if v_dst.shape != k_dst.shape:
-                raise ValueError("k_dst and v_dst must have the same shape.")
-        psl, pages, psize = _vec(slots, "slots", dev, _I64, R), k_dst.shape[0], k_dst.shape[1]
-        kst = k_dst.stride()[:3]
-        vst = (0, 0, 0) if v is None else v_dst.stride()[:3]
-    wt = tt = dt
-    pw = [0, 0]
-    for i, (w, name) in enumerate(((q_weight, "q_weight"), (k_weight, "k_weight"))):
-        if w is not None:
-            if not isinstance(w, torch.Tensor) or w.dtype not in (dt, torch.float32):
-                raise ValueError(f"{name} must be a tensor of {dt} or float32.")
-            wt = w.dtype
-            pw[i] = _vec(w, name, dev, wt, hd)
-    if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
-        raise ValueError("q_weight and k_weight must have the same type.")
-    pc = psn = cst = sst = trows = rot = 0
+        if k_dst.dim() != 4:
+            raise ValueError("with slots k_dst and v_dst must be [pages, page_size, kv_heads, head_dim].")
+        pages, psize = k_dst.shape[:2]
+        dst, psl = (pages, psize, nkv, hd), _vec(slots, "slots", index, _I64, R)
+    kd = _rows(k_dst, "k_dst", index, kt, dst)
+    _apart(q_out, os, "q_out")
+    _apart(k_dst, kd, "k_dst")
+    vs, vd, pv, pvd = (0, 0), kd, 0, 0
+    if v is not None:
+        vs, vd = _rows(v, "v", index, dt, kv_shape), _rows(v_dst, "v_dst", index, kt, dst)
+        _apart(v_dst, vd, "v_dst")
+        pv, pvd = v.data_ptr(), v_dst.data_ptr()
+    if slots is None:
+        kd, vd = (kd[0], 0, kd[1]), (vd[0], 0, vd[1])
+    wt, pqw, pkw = dt, 0, 0
+    if q_weight is not None:
+        wt = q_weight.dtype
+        pqw = _vec(q_weight, "q_weight", index, wt, hd)
+    if k_weight is not None:
+        if q_weight is None:
+            wt = k_weight.dtype
+        pkw = _vec(k_weight, "k_weight", index, wt, hd)  # of one type with q_weight
+    tt, pc, psn, cst, sst, trows, rot = dt, 0, 0, 0, 0, 0, 0
     if (cos is None) != (sin is None):
         raise ValueError("cos and sin come together.")
     if cos is not None:
-        if not isinstance(cos, torch.Tensor) or cos.dim() != 2 or cos.dtype not in (dt, torch.float32):
-            raise ValueError(f"cos must be {dt} or float32 [table rows, rot_dim / 2].")
-        tt, trows, rot = cos.dtype, cos.shape[0], 2 * cos.shape[1]
-        for t, name in ((cos, "cos"), (sin, "sin")):
-            if not isinstance(t, torch.Tensor) or t.device != dev or t.dtype != tt or t.shape != cos.shape or \
-                    _gaps(t):
-                raise ValueError(f"{name} must be {tt} {tuple(cos.shape)} on {dev} with contiguous rows.")
-        pc, psn, cst, sst = cos.data_ptr(), sin.data_ptr(), cos.stride(0), sin.stride(0)
-        if rot == 0:
-            pc = psn = 0
+        tt = cos.dtype
+        trows, half = cos.shape
+        cst, sst = _rows(cos, "cos", index, tt, cos.shape)[0], _rows(sin, "sin", index, tt, cos.shape)[0]
+        rot = 2 * half
+        if rot:
+            pc, psn = cos.data_ptr(), sin.data_ptr()
+    if (wt is not dt and wt is not _F32) or (tt is not dt and tt is not _F32):
+        raise ValueError(f"weights and tables must be {dt} or float32.")
     ppos, p64 = 0, 0
     if positions is not None:
-        p64 = 1 if isinstance(positions, torch.Tensor) and positions.dtype == _I64 else 0
-        ppos = _vec(positions, "positions", dev, _I64 if p64 else _I32, R)
+        p64 = 1 if positions.dtype is _I64 else 0
+        ppos = _vec(positions, "positions", index, _I64 if p64 else _I32, R)
     if R == 0:
         return
-    packed = _ROPE.pack(pq, pk, pv, po, pkd, pvd, pw[0], pw[1], pc, psn, ppos, psl, q.stride(0), q.stride(1), k.stride(0),
-                        k.stride(1), v.stride(0) if pv else 0, v.stride(1) if pv else 0, q_out.stride(0), q_out.stride(1),
-                        *kst, *vst, cst, sst, trows, pages, R, nq, nkv, hd, rot, psize, _DT[dt], _DT[q_out.dtype], _DT[kt],
-                        _DT[wt], _DT[tt], p64, float(eps), 0)
-    _run(lib().tt_qk_norm_rope, packed, dev, "qk_norm_rope")
+    packed = _ROPE.pack(q.data_ptr(), k.data_ptr(), pv, q_out.data_ptr(), k_dst.data_ptr(), pvd, pqw, pkw, pc, psn, ppos, psl,
+                        qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os[0], os[1], kd[0], kd[1], kd[2], vd[0], vd[1], vd[2], cst, sst,
+                        trows, pages, R, nq, nkv, hd, rot, psize, _DT[dt], _DT[qt], _DT[kt], _DT[wt], _DT[tt], p64, eps, 0)
+    _run(lib().tt_qk_norm_rope, packed, index, "qk_norm_rope")
 
 
+@_tensors_only
 def shared_prefix_attention(q, k_pages, v_pages, prefix_table, prefix_len, tables, row_lens, out, row_seq=None,
                             scale=None) -> None:
     """Decode attention of a batch over a prefix that all rows share, read once
@@ -223,51 +221,50 @@ def shared_prefix_attention(q, k_pages, v_pages, prefix_table, prefix_len, table
     they were; a row with nothing to attend gives zeros; a page outside the pool
     or a length beyond the table gives NaN.  out may be q itself.
     """
-    dev = _device(q, "q")
+    index = _device(q, "q")
     dt = q.dtype
-    if dt not in (torch.bfloat16, torch.float16) or q.dim() != 3:
+    if (dt is not _BF16 and dt is not _F16) or q.dim() != 3:
         raise ValueError("q must be bfloat16 or float16 [rows, heads, head_dim].")
-    R, nq, hd = q.shape
-    if not isinstance(k_pages, torch.Tensor) or k_pages.dim() != 4:
-        raise ValueError("k_pages must be a tensor [pages, page_size, kv_heads, head_dim].")
-    nkv = k_pages.shape[2]
-    pq, po = _heads(q, "q", dev, dt, R, nq, hd), _heads(out, "out", dev, dt, R, nq, hd)
-    _apart(out, "out")
-    pk, pv = _pool(k_pages, "k_pages", dev, dt, nkv, hd), _pool(v_pages, "v_pages", dev, dt, nkv, hd)
-    if v_pages.shape != k_pages.shape:
-        raise ValueError("k_pages and v_pages must have the same shape.")
+    R, nq, hd = shape = q.shape
+    if k_pages.dim() != 4 or k_pages.shape[3] != hd:
+        raise ValueError(f"k_pages must be [pages, page_size, kv_heads, {hd}].")
+    pages, P, nkv, _ = pool = k_pages.shape
     if nq == 0 or nkv == 0 or nq % nkv:
         raise ValueError("the query heads must be a positive multiple of the kv heads.")
-    prefix_len = int(prefix_len)
-    P = k_pages.shape[1]
-    ppt = _vec(prefix_table, "prefix_table", dev, _I32) if prefix_table is not None else 0
-    if prefix_len < 0 or (prefix_len and (not ppt or prefix_table.shape[0] * P < prefix_len)):
+    qs, os = _rows(q, "q", index, dt, shape), _rows(out, "out", index, dt, shape)
+    _apart(out, os, "out")
+    ks, vs = _rows(k_pages, "k_pages", index, dt, pool), _rows(v_pages, "v_pages", index, dt, pool)
+    if 1 in pool:  # the stride of a dimension of one entry says nothing
+        ks, vs = (tuple(d if n > 1 else hd for n, d in zip(pool, st)) for st in (ks, vs))
+    ppt, have = 0, 0
+    if prefix_table is not None:
+        have = prefix_table.numel()
+        ppt = _vec(prefix_table, "prefix_table", index, _I32, have)
+    if prefix_len < 0 or have * P < prefix_len:
         raise ValueError("prefix_table does not hold prefix_len tokens.")
-    if not isinstance(tables, torch.Tensor) or tables.device != dev or tables.dtype != _I32 or tables.dim() != 2 or \
-            _gaps(tables):
-        raise ValueError(f"tables must be int32 [requests, width] on {dev} with contiguous rows.")
+    if tables.dim() != 2:
+        raise ValueError("tables must be int32 [requests, width].")
     B, W = tables.shape
-    pl = _vec(row_lens, "row_lens", dev, _I32, R)
-    prs = 0
-    if row_seq is not None:
-        prs = _vec(row_seq, "row_seq", dev, _I32, R)
-    elif B < R:
+    ts = _rows(tables, "tables", index, _I32, tables.shape)
+    pl = _vec(row_lens, "row_lens", index, _I32, R)
+    prs = 0 if row_seq is None else _vec(row_seq, "row_seq", index, _I32, R)
+    if row_seq is None and B < R:
         raise ValueError("without row_seq the tables need a row for each row.")
     if R == 0:
         return
-    scale = hd ** -0.5 if scale is None else float(scale)
+    scale = hd ** -0.5 if scale is None else scale
     if not math.isfinite(scale):
         raise ValueError("scale must be finite.")
-    # the stride of a dimension of one entry says nothing
-    ks, vs = (tuple(st if n > 1 else hd for n, st in zip(t.shape, t.stride())) for t in (k_pages, v_pages))
-    rest = (q.stride(0), q.stride(1), out.stride(0), out.stride(1), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], tables.stride(0),
-            R, nq, nkv, hd, P, k_pages.shape[0], prefix_len, W, B, _DT[dt], scale, 0)
+    first = (q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), ppt, tables.data_ptr(), pl, prs)
+    rest = (qs[0], qs[1], os[0], os[1], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], ts[0], R, nq, nkv, hd, P, pages, prefix_len, W, B,
+            1 if dt is _BF16 else 2, scale, 0)
     L = lib()
-    size = C.c_size_t()
-    st = L.tt_shared_prefix_attention_workspace(_PREFIX.pack(pq, pk, pv, po, ppt, tables.data_ptr(), pl, prs, 0, *rest),
-                                                C.byref(size))
+    size = getattr(_local, "size", None)
+    if size is None:
+        size = _local.size = C.c_size_t()
+    st = L.tt_shared_prefix_attention_workspace(_PREFIX.pack(*first, 0, *rest), C.byref(size))
     if st:
         check(st, "shared_prefix_attention")
-    ws = torch.empty(size.value, dtype=torch.uint8, device=dev) if size.value else None
-    _run(L.tt_shared_prefix_attention, _PREFIX.pack(pq, pk, pv, po, ppt, tables.data_ptr(), pl, prs,
-                                                    0 if ws is None else ws.data_ptr(), *rest), dev, "shared_prefix_attention")
+    ws = torch.empty(size.value, dtype=torch.uint8, device=q.device) if size.value else None
+    _run(L.tt_shared_prefix_attention, _PREFIX.pack(*first, 0 if ws is None else ws.data_ptr(), *rest), index,
+         "shared_prefix_attention")
