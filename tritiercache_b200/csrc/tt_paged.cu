@@ -64,6 +64,12 @@ __device__ __forceinline__ Pair64 block_scan2(Pair64 v, Pair64* tot, Pair64* sm)
 
 __device__ __forceinline__ int clamp_i32(long long x) { return x > INT_MAX ? INT_MAX : (int)x; }
 
+// Pages that hold x tokens (x below 2^32).
+__device__ __forceinline__ int pt_pages(const tt_page_tables_args& p, long long x) {
+    const uint32_t u = (uint32_t)x, P = (uint32_t)p.page_size;
+    return (int)(u / P) + (u % P != 0);
+}
+
 struct PtReq {
     long long ctx, held, n;  // tokens held, pages held, new tokens
     bool ended;
@@ -73,7 +79,7 @@ __device__ __forceinline__ PtReq pt_req(const tt_page_tables_args& p, int b) {
     if (b < p.num_seqs) {
         const int c = p.ctx_lens[b], n = p.new_lens[b];
         r.ctx = c > 0 ? c : 0;
-        r.held = (r.ctx + p.page_size - 1) / p.page_size;
+        r.held = pt_pages(p, r.ctx);
         r.ended = n < 0;
         r.n = n > 0 ? n : 0;
     }
@@ -88,7 +94,7 @@ struct PtRow {
 __device__ __forceinline__ PtRow pt_row(const tt_page_tables_args& p, int b, int ctx, int cu, int first, int top,
                                         int t) {
     if (first < 0) return PtRow{-1, 0, -1, 0};
-    const int held = (int)(((long long)ctx + p.page_size - 1) / p.page_size);
+    const int held = pt_pages(p, ctx);
     const int pos = ctx + (t - cu), pg = pos / p.page_size;
     const int page = pg < held ? p.tables[b * p.table_stride + pg] : p.free_pages[top - 1 - first - (pg - held)];
     return PtRow{(long long)page * p.page_size + pos % p.page_size, pos + p.position_offset, b, pos + 1};
@@ -189,7 +195,7 @@ __global__ void __launch_bounds__(kPtThreads) k_page_scan(const tt_page_tables_a
         for (int i = 0; i < kPtItems; ++i) {
             const int b = base + tid * kPtItems + i;
             r[i] = pt_req(p, b);
-            const long long last = (r[i].ctx + r[i].n + p.page_size - 1) / p.page_size;
+            const long long last = pt_pages(p, r[i].ctx + r[i].n);
             const long long end = b < B ? (long long)(SMALL ? cu_s[b] : p.cu_new[b]) + r[i].n : 0;
             late[i] = r[i].n > 0 && (last > p.table_width || end > p.num_rows);
             need[i] = r[i].n > 0 && !late[i] ? (int)(last - r[i].held) : 0;
@@ -246,7 +252,7 @@ __global__ void __launch_bounds__(kPtThreads) k_page_scan(const tt_page_tables_a
 constexpr int kPrThreads = 256;
 constexpr int kPrRows = 4;  // consecutive rows per thread: one search, 16- and 32-byte stores
 
-__global__ void __launch_bounds__(kPrThreads) k_page_rows(const tt_page_tables_args p, int row_blocks) {
+__global__ void __launch_bounds__(kPrThreads) k_page_rows(const tt_page_tables_args p, int row_blocks, int wide) {
     pdl_wait();
     const int B = p.num_seqs, top = static_cast<const PtWorkspace*>(p.workspace)->top;
     const int* first = reinterpret_cast<const int*>(static_cast<const PtWorkspace*>(p.workspace) + 1);
@@ -255,11 +261,23 @@ __global__ void __launch_bounds__(kPrThreads) k_page_rows(const tt_page_tables_a
         const long long t0 = ((long long)blockIdx.x * kPrThreads + threadIdx.x) * kPrRows;
         if (t0 >= p.num_rows) return;
         int b = pt_find([&](int i) { return p.cu_new[i]; }, B, (int)t0);
+        PtRow r[kPrRows];
+#pragma unroll
         for (int i = 0; i < kPrRows; ++i) {
             const long long t = t0 + i;
-            if (t >= p.num_rows) break;
             while (b < B && p.cu_new[b + 1] <= t) ++b;
-            pt_store(p, (int)t, b < B ? pt_row(p, b, ctx[b], p.cu_new[b], first[b], top, (int)t) : PtRow{-1, 0, -1, 0});
+            r[i] = b < B ? pt_row(p, b, ctx[b], p.cu_new[b], first[b], top, (int)t) : PtRow{-1, 0, -1, 0};
+        }
+        if (t0 + kPrRows <= p.num_rows && wide) {
+            reinterpret_cast<longlong2*>(p.slots + t0)[0] = make_longlong2(r[0].slot, r[1].slot);
+            reinterpret_cast<longlong2*>(p.slots + t0)[1] = make_longlong2(r[2].slot, r[3].slot);
+            *reinterpret_cast<int4*>(p.positions + t0) = make_int4(r[0].pos, r[1].pos, r[2].pos, r[3].pos);
+            *reinterpret_cast<int4*>(p.row_seq + t0) = make_int4(r[0].seq, r[1].seq, r[2].seq, r[3].seq);
+            *reinterpret_cast<int4*>(p.row_lens + t0) = make_int4(r[0].len, r[1].len, r[2].len, r[3].len);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kPrRows; ++i)
+                if (t0 + i < p.num_rows) pt_store(p, (int)(t0 + i), r[i]);
         }
     } else {
         const int w = ((blockIdx.x - row_blocks) * kPrThreads + threadIdx.x) >> 5, lane = threadIdx.x & 31;
@@ -267,8 +285,7 @@ __global__ void __launch_bounds__(kPrThreads) k_page_rows(const tt_page_tables_a
         for (int b = w; b < B; b += nw) {
             const int n = p.new_lens[b];
             if (first[b] < 0 || n <= 0) continue;
-            const int held = (int)(((long long)ctx[b] + p.page_size - 1) / p.page_size);
-            const int given = (int)(((long long)ctx[b] + n + p.page_size - 1) / p.page_size) - held;
+            const int held = pt_pages(p, ctx[b]), given = pt_pages(p, (long long)ctx[b] + n) - held;
             for (int j = lane; j < given; j += 32)
                 p.tables[b * p.table_stride + held + j] = p.free_pages[top - 1 - first[b] - j];
         }
@@ -281,10 +298,11 @@ __global__ void __launch_bounds__(kPrThreads) k_page_rows(const tt_page_tables_a
 // A head's hd/2 channel pairs (c, c + rot/2), or (c, c + (hd-rot)/2) behind rot, are spread over G lanes,
 // VEC consecutive pairs a lane and step, so both channels of a pair meet in one lane, loads are 2 x VEC
 // contiguous elements, and the sum of squares is one butterfly over G lanes.  A group of G lanes keeps the
-// cos, sin and weights of its channels in registers and walks `chunk` heads of one row, so the tables are
-// read once a row and chunk, not once a head.  Bytes of q, k, v in and out are the floor.
+// cos, sin and weights of its channels in registers and walks up to `chunk` heads of one kind (query, key or
+// value) of one row, so the tables are read once a row and chunk, not once a head, and it asks for `kBatch`
+// heads before it works on the first.  Bytes of q, k, v in and out are the floor.
 // ---------------------------------------------------------------------------
-template <typename T> struct Elem;
+template <typename T> struct Elem;  // float32 of a value and back, one at a time and as the halves of a word
 template <> struct Elem<float> {
     static __device__ __forceinline__ float up(float x) { return x; }
     static __device__ __forceinline__ float down(float x) { return x; }
@@ -292,140 +310,271 @@ template <> struct Elem<float> {
 template <> struct Elem<__nv_bfloat16> {
     static __device__ __forceinline__ float up(__nv_bfloat16 x) { return __bfloat162float(x); }
     static __device__ __forceinline__ __nv_bfloat16 down(float x) { return __float2bfloat16_rn(x); }
+    static __device__ __forceinline__ float2 up2(uint32_t w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
+    static __device__ __forceinline__ uint32_t down2(float x, float y) {
+        uint32_t r;
+        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(y), "f"(x));
+        return r;
+    }
 };
 template <> struct Elem<__half> {
     static __device__ __forceinline__ float up(__half x) { return __half2float(x); }
     static __device__ __forceinline__ __half down(float x) { return __float2half_rn(x); }
+    static __device__ __forceinline__ float2 up2(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+    static __device__ __forceinline__ uint32_t down2(float x, float y) {
+        uint32_t r;
+        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(y), "f"(x));
+        return r;
+    }
 };
 
-template <typename T, int N>
-struct alignas(sizeof(T) * N <= 16 ? sizeof(T) * N : 16) Pack {
-    T x[N];
+// N values of T as the 16-byte words that memory moves them in (arrays of 16-bit classes are moved one by one);
+// N = 1 is the unaligned form.
+template <typename T, int N> struct Pack {
+    static constexpr int kWords = N * (int)sizeof(T) / 16;
+    uint4 w[kWords];
+    __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+        for (int k = 0; k < kWords; ++k) w[k] = reinterpret_cast<const uint4*>(p)[k];
+    }
+    __device__ __forceinline__ void store(T* p) const {
+#pragma unroll
+        for (int k = 0; k < kWords; ++k) reinterpret_cast<uint4*>(p)[k] = w[k];
+    }
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int k = 0; k < kWords; ++k) w[k] = make_uint4(0, 0, 0, 0);
+    }
+    __device__ __forceinline__ void up(float* f) const {
+#pragma unroll
+        for (int k = 0; k < kWords; ++k) {
+            const uint32_t v[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (sizeof(T) == 4) {
+                    f[4 * k + i] = __uint_as_float(v[i]);
+                } else {
+                    const float2 x = Elem<T>::up2(v[i]);
+                    f[8 * k + 2 * i] = x.x;
+                    f[8 * k + 2 * i + 1] = x.y;
+                }
+            }
+        }
+    }
+    __device__ __forceinline__ void down(const float* f) {
+#pragma unroll
+        for (int k = 0; k < kWords; ++k) {
+            uint32_t v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (sizeof(T) == 4) v[i] = __float_as_uint(f[4 * k + i]);
+                else v[i] = Elem<T>::down2(f[8 * k + 2 * i], f[8 * k + 2 * i + 1]);
+            }
+            w[k] = make_uint4(v[0], v[1], v[2], v[3]);
+        }
+    }
 };
+template <typename T> struct Pack<T, 1> {
+    T x;
+    __device__ __forceinline__ void load(const T* p) { x = *p; }
+    __device__ __forceinline__ void store(T* p) const { *p = x; }
+    __device__ __forceinline__ void zero() { x = Elem<T>::down(0.f); }
+    __device__ __forceinline__ void up(float* f) const { *f = Elem<T>::up(x); }
+    __device__ __forceinline__ void down(const float* f) { x = Elem<T>::down(*f); }
+};
+
+// x += a b, y += c d in one instruction
+__device__ __forceinline__ void fma2(float& x, float& y, float a, float c, float b, float d) {
+    asm("{\n.reg .b64 v, a, b;\nmov.b64 v, {%0, %1};\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %5};\n"
+        "fma.rn.f32x2 v, a, b, v;\nmov.b64 {%0, %1}, v;\n}" : "+f"(x), "+f"(y) : "f"(a), "f"(c), "f"(b), "f"(d));
+}
 
 template <typename T, int VEC>
 __device__ __forceinline__ void load_pack(const T* p, float* f) {
-    const Pack<T, VEC> v = *reinterpret_cast<const Pack<T, VEC>*>(p);
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) f[i] = Elem<T>::up(v.x[i]);
+    Pack<T, VEC> v;
+    v.load(p);
+    v.up(f);
 }
 template <typename T, int VEC>
 __device__ __forceinline__ void store_pack(T* p, const float* f) {
     Pack<T, VEC> v;
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) v.x[i] = Elem<T>::down(f[i]);
-    *reinterpret_cast<Pack<T, VEC>*>(p) = v;
+    v.down(f);
+    v.store(p);
 }
 template <typename T>
 __device__ __forceinline__ float load_any(const void* p, long long i, bool f32) {
     return f32 ? static_cast<const float*>(p)[i] : Elem<T>::up(static_cast<const T*>(p)[i]);
 }
 
-template <typename T, typename TQ, typename TKV, int VEC, int STEPS>
-__global__ void __launch_bounds__(256) k_norm_rope(const tt_qk_norm_rope_args p, int glog, int chunk, int chunks) {
-    const int G = 1 << glog, lane = threadIdx.x & (G - 1);
-    const long long item = ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> glog;
-    const long long row = item / chunks;
-    // groups past the end keep running (the butterflies are warp-wide) without loads or stores
-    const bool in = row < p.num_rows;
-    const int h0 = (int)(item % chunks) * chunk;
-    const int heads = p.num_q_heads + (p.v ? 2 : 1) * p.num_kv_heads;
+// N values of T or float32 from p[i] on; `aligned` when 16-byte loads may be used.
+template <typename T, int N>
+__device__ __forceinline__ void load_row(const void* p, long long i, bool f32, bool aligned, float* f) {
+    if (N > 1 && aligned) {
+        if (f32) load_pack<float, N>(static_cast<const float*>(p) + i, f);
+        else load_pack<T, N>(static_cast<const T*>(p) + i, f);
+    } else {
+#pragma unroll
+        for (int k = 0; k < N; ++k) f[k] = load_any<T>(p, i + k, f32);
+    }
+}
+
+// Measured for 32k rows of 32 + 8 + 8 heads of 128 (floor 125 us at the copy rate): batches of 1, 2, 4, 8 heads
+// 240, 200, 177, 280 us (one head leaves too little in flight, eight spend the registers that warps need);
+// 4, 8, 16 heads a group 230 (batch 2), 177, 187; blocks of 256 and 128 threads 177, 172.
+constexpr int kNrChunk = 8, kNrBatch = 4, kNrThreads = 1024, kNrBlock = 128;
+
+// Groups of a row: cq for the queries, then ck for the keys, then (with v) ck for the values; group c of a kind
+// takes heads c, c + cq (or ck), ..., so that the groups of a warp are at neighbouring heads together.
+struct NrShape {
+    int glog, chunk, cq, ck, chunks;
+    int table_aligned, weight_aligned;
+};
+
+// With a row's cos, sin and a head's weights, x' = r (A x - B y) and y' = r (C y + D x) for each pair, where
+// A = w_x cos, B = w_y sin, C = w_y cos, D = w_x sin and r = rsqrt(mean square + eps).  FULL: every channel is
+// rotated (else the others take x' = r A x, without the partner, which may be infinite).
+template <typename T, typename TQ, typename TKV, int VEC, int STEPS, int kBatch, bool FULL>
+__global__ void __launch_bounds__(kNrBlock) k_norm_rope(const tt_qk_norm_rope_args p, const NrShape sh) {
+    const int G = 1 << sh.glog, lane = threadIdx.x & (G - 1);
+    const long long item = ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> sh.glog;
+    const long long row = item / sh.chunks;
+    const int ch = (int)(item % sh.chunks);
+    const int kind = ch < sh.cq ? 0 : ch < sh.cq + sh.ck ? 1 : 2;
+    const int h0 = kind == 0 ? ch : kind == 1 ? ch - sh.cq : ch - sh.cq - sh.ck, hstep = kind == 0 ? sh.cq : sh.ck;
     const int hd = p.head_dim, half = p.rot_dim >> 1, rest = (hd - p.rot_dim) >> 1;
 
-    bool live = in;
+    // groups past the end keep running (the butterflies are warp-wide) without loads or stores
+    bool live = row < p.num_rows;
     long long page = row;
     int tok = 0;
-    if (in && p.slots) {
+    if (live && p.slots) {
         const long long s = p.slots[row];
         live = s >= 0 && s < p.num_pages * p.page_size;
         page = s / p.page_size;
         tok = (int)(s % p.page_size);
     }
-    long long pos = row;
-    if (in && p.positions) pos = p.positions_i64 ? static_cast<const long long*>(p.positions)[row]
-                                                 : (long long)static_cast<const int*>(p.positions)[row];
-    const bool pos_ok = pos >= 0 && pos < p.table_rows;
+    // this group's heads: h0, h0 + hstep, ...
+    const int mine = live ? ((kind == 0 ? p.num_q_heads : p.num_kv_heads) - h0 + hstep - 1) / hstep : 0;
+    const T* src = kind == 0 ? static_cast<const T*>(p.q) + row * p.q_row_stride + h0 * p.q_head_stride
+                 : kind == 1 ? static_cast<const T*>(p.k) + row * p.k_row_stride + h0 * p.k_head_stride
+                             : static_cast<const T*>(p.v) + row * p.v_row_stride + h0 * p.v_head_stride;
+    const long long src_step = hstep * (kind == 0 ? p.q_head_stride : kind == 1 ? p.k_head_stride : p.v_head_stride);
+    TQ* dq = static_cast<TQ*>(p.q_out) + row * p.q_out_row_stride + h0 * p.q_out_head_stride;
+    TKV* dkv = kind == 1 ? static_cast<TKV*>(p.k_dst) + page * p.k_page_stride + tok * p.k_token_stride + h0 * p.k_dst_head_stride
+                         : static_cast<TKV*>(p.v_dst) + page * p.v_page_stride + tok * p.v_token_stride + h0 * p.v_dst_head_stride;
+    const long long dst_step = hstep * (kind == 0 ? p.q_out_head_stride : kind == 1 ? p.k_dst_head_stride : p.v_dst_head_stride);
 
     int ca[STEPS], cb[STEPS];  // first channels of this lane's runs of pairs, -1: none
-    float co[STEPS][VEC], si[STEPS][VEC], wq[2][STEPS][VEC], wk[2][STEPS][VEC];
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) {
         const int pr = (lane + s * G) * VEC;
         ca[s] = pr < half ? pr : pr < half + rest ? pr + half : -1;
         cb[s] = pr < half ? pr + half : ca[s] + rest;
+    }
+    // the first heads are on their way before the tables are asked for
+    Pack<T, VEC> ra[kBatch][STEPS], rb[kBatch][STEPS];
+    const auto fetch = [&](int i) {
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+#pragma unroll
+            for (int s = 0; s < STEPS; ++s) {
+                if (i + u < mine && ca[s] >= 0) {
+                    ra[u][s].load(src + ca[s]);
+                    rb[u][s].load(src + cb[s]);
+                } else {
+                    ra[u][s].zero();
+                    rb[u][s].zero();
+                }
+            }
+            src += src_step;
+        }
+    };
+    fetch(0);
+
+    const void* weight = kind == 0 ? p.q_weight : kind == 1 ? p.k_weight : nullptr;
+    float A[STEPS][VEC], B[STEPS][VEC], C[STEPS][VEC], D[STEPS][VEC];
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+        float co[VEC], si[VEC], wa[VEC], wb[VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) co[i] = wa[i] = wb[i] = 1.f, si[i] = 0.f;
+        const int pr = (lane + s * G) * VEC;
+        if (mine > 0 && kind < 2 && pr < half) {
+            long long pos = row;
+            if (p.positions) pos = p.positions_i64 ? static_cast<const long long*>(p.positions)[row]
+                                                   : (long long)static_cast<const int*>(p.positions)[row];
+            const bool f32 = p.table_dtype == TT_DTYPE_F32;
+            if (pos >= 0 && pos < p.table_rows) {
+                load_row<T, VEC>(p.cos, pos * p.cos_stride + pr, f32, sh.table_aligned, co);
+                load_row<T, VEC>(p.sin, pos * p.sin_stride + pr, f32, sh.table_aligned, si);
+            } else {
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) co[i] = si[i] = NAN;
+            }
+        }
+        if (mine > 0 && weight && ca[s] >= 0) {
+            const bool f32 = p.weight_dtype == TT_DTYPE_F32;
+            load_row<T, VEC>(weight, ca[s], f32, sh.weight_aligned, wa);
+            load_row<T, VEC>(weight, cb[s], f32, sh.weight_aligned, wb);
+        }
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
-            co[s][i] = 1.f;
-            si[s][i] = 0.f;
-            if (live && pr < half) {
-                co[s][i] = pos_ok ? load_any<T>(p.cos, pos * p.cos_stride + pr + i, p.table_dtype == TT_DTYPE_F32) : NAN;
-                si[s][i] = pos_ok ? load_any<T>(p.sin, pos * p.sin_stride + pr + i, p.table_dtype == TT_DTYPE_F32) : NAN;
-            }
-            const bool use = live && ca[s] >= 0, f = p.weight_dtype == TT_DTYPE_F32;
-            wq[0][s][i] = use && p.q_weight ? load_any<T>(p.q_weight, ca[s] + i, f) : 1.f;
-            wq[1][s][i] = use && p.q_weight ? load_any<T>(p.q_weight, cb[s] + i, f) : 1.f;
-            wk[0][s][i] = use && p.k_weight ? load_any<T>(p.k_weight, ca[s] + i, f) : 1.f;
-            wk[1][s][i] = use && p.k_weight ? load_any<T>(p.k_weight, cb[s] + i, f) : 1.f;
+            A[s][i] = wa[i] * co[i];
+            B[s][i] = wb[i] * si[i];
+            C[s][i] = wb[i] * co[i];
+            D[s][i] = wa[i] * si[i];
         }
     }
     const float inv = 1.f / (float)hd;
 
-#pragma unroll 2
-    for (int hh = 0; hh < chunk; ++hh) {
-        const int h = h0 + hh;
-        const bool is_q = h < p.num_q_heads, is_k = !is_q && h < p.num_q_heads + p.num_kv_heads;
-        const bool on = live && h < heads;
-        const int kh = is_q ? h : is_k ? h - p.num_q_heads : h - p.num_q_heads - p.num_kv_heads;
-        const T* src = is_q ? static_cast<const T*>(p.q) + row * p.q_row_stride + kh * p.q_head_stride
-                     : is_k ? static_cast<const T*>(p.k) + row * p.k_row_stride + kh * p.k_head_stride
-                            : static_cast<const T*>(p.v) + row * p.v_row_stride + kh * p.v_head_stride;
-        float a[STEPS][VEC], b[STEPS][VEC];
-        float ss = 0.f;
+    for (int i = 0; i < sh.chunk; i += kBatch) {
+        if (i) fetch(i);
 #pragma unroll
-        for (int s = 0; s < STEPS; ++s) {
-            if (on && ca[s] >= 0) {
-                load_pack<T, VEC>(src + ca[s], a[s]);
-                load_pack<T, VEC>(src + cb[s], b[s]);
-            } else {
+        for (int u = 0; u < kBatch; ++u) {
+            float a[STEPS][VEC], b[STEPS][VEC], s0 = 0.f, s1 = 0.f;
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) a[s][i] = b[s][i] = 0.f;
+            for (int s = 0; s < STEPS; ++s) {
+                ra[u][s].up(a[s]);
+                rb[u][s].up(b[s]);
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) fma2(s0, s1, a[s][k], b[s][k], a[s][k], b[s][k]);
             }
+            // groups of one warp may be at heads of different kinds: all lanes take the butterfly
+            float ss = s0 + s1;
+            for (int d = G >> 1; d; d >>= 1) ss += __shfl_xor_sync(~0u, ss, d);
+            const float r = weight ? rsqrtf(ss * inv + p.eps) : 1.f;
+            if (i + u < mine) {
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) ss += a[s][i] * a[s][i] + b[s][i] * b[s][i];
-        }
-        // groups of one warp may be at heads of different kinds: all lanes take the butterfly
-        for (int d = G >> 1; d; d >>= 1) ss += __shfl_xor_sync(~0u, ss, d);
-        if (is_q ? p.q_weight != nullptr : is_k && p.k_weight != nullptr) {
-            const float r = rsqrtf(ss * inv + p.eps);
+                for (int s = 0; s < STEPS; ++s) {
+                    if (ca[s] < 0) continue;
+                    float x[VEC], y[VEC];
+                    if (kind < 2) {
 #pragma unroll
-            for (int s = 0; s < STEPS; ++s)
+                        for (int k = 0; k < VEC; ++k) {
+                            x[k] = A[s][k] * a[s][k];
+                            y[k] = C[s][k] * b[s][k];
+                            if (FULL || ca[s] < half) {
+                                x[k] = fmaf(-B[s][k], b[s][k], x[k]);
+                                y[k] = fmaf(D[s][k], a[s][k], y[k]);
+                            }
+                            x[k] *= r;
+                            y[k] *= r;
+                        }
+                    } else {
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) {
-                    a[s][i] *= r * (is_q ? wq[0][s][i] : wk[0][s][i]);
-                    b[s][i] *= r * (is_q ? wq[1][s][i] : wk[1][s][i]);
+                        for (int k = 0; k < VEC; ++k) x[k] = a[s][k], y[k] = b[s][k];
+                    }
+                    if (kind == 0) {
+                        store_pack<TQ, VEC>(dq + ca[s], x);
+                        store_pack<TQ, VEC>(dq + cb[s], y);
+                    } else {
+                        store_pack<TKV, VEC>(dkv + ca[s], x);
+                        store_pack<TKV, VEC>(dkv + cb[s], y);
+                    }
                 }
-        }
-        if (!on) continue;
-#pragma unroll
-        for (int s = 0; s < STEPS; ++s) {
-            if (ca[s] < 0) continue;
-            float x[VEC], y[VEC];
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                const bool turn = (is_q || is_k) && ca[s] < half;
-                x[i] = turn ? a[s][i] * co[s][i] - b[s][i] * si[s][i] : a[s][i];
-                y[i] = turn ? b[s][i] * co[s][i] + a[s][i] * si[s][i] : b[s][i];
             }
-            if (is_q) {
-                TQ* d = static_cast<TQ*>(p.q_out) + row * p.q_out_row_stride + kh * p.q_out_head_stride;
-                store_pack<TQ, VEC>(d + ca[s], x);
-                store_pack<TQ, VEC>(d + cb[s], y);
-            } else {
-                TKV* d = is_k ? static_cast<TKV*>(p.k_dst) + page * p.k_page_stride + tok * p.k_token_stride + kh * p.k_dst_head_stride
-                              : static_cast<TKV*>(p.v_dst) + page * p.v_page_stride + tok * p.v_token_stride + kh * p.v_dst_head_stride;
-                store_pack<TKV, VEC>(d + ca[s], x);
-                store_pack<TKV, VEC>(d + cb[s], y);
-            }
+            dq += dst_step;
+            dkv += dst_step;
         }
     }
 }
@@ -434,20 +583,26 @@ template <typename T, typename TQ, typename TKV>
 static cudaError_t launch_norm_rope(const tt_qk_norm_rope_args& a, bool vec, cudaStream_t st) {
     constexpr int V = 16 / sizeof(T);
     const int pairs = a.head_dim / 2, width = vec ? V : 1;
-    int glog = 0;
-    while (glog < 5 && (1 << glog) * width < pairs) ++glog;
-    const int G = 1 << glog, steps = (pairs + G * width - 1) / (G * width);
-    // Heads a group walks: as many as leave about four warps an SM partition, so that tables and weights
-    // are read seldom in a long prompt and a single token still uses a group per head.
-    const int heads = a.num_q_heads + (a.v ? 2 : 1) * a.num_kv_heads;
-    int chunk = heads;
-    while (chunk > 1 && (long long)a.num_rows * ((heads + chunk - 1) / chunk) * G < 148LL * 512) chunk = (chunk + 1) / 2;
-    const int chunks = (heads + chunk - 1) / chunk;
-    const long long threads = (long long)a.num_rows * chunks * G;
-    const dim3 grid((unsigned)((threads + 255) / 256)), block(256);
-#define TT_NR(VV, SS) launch(k_norm_rope<T, TQ, TKV, VV, SS>, grid, block, 0, st, false, a, glog, chunk, chunks)
-    if (vec) return steps <= 1 ? TT_NR(V, 1) : TT_NR(V, 2);
-    return steps <= 2 ? TT_NR(1, 2) : TT_NR(1, 8);
+    NrShape sh = {};
+    while (sh.glog < 5 && (1 << sh.glog) * width < pairs) ++sh.glog;
+    const int G = 1 << sh.glog, steps = (pairs + G * width - 1) / (G * width);
+    // Heads a group walks: up to kNrChunk, fewer while the groups would not fill the GPU, so that a single token
+    // uses a group per head.
+    const auto chunks = [&](int c) { return (a.num_q_heads + c - 1) / c + (a.v ? 2 : 1) * ((a.num_kv_heads + c - 1) / c); };
+    sh.chunk = kNrChunk;
+    while (sh.chunk > 1 && (long long)a.num_rows * chunks(sh.chunk) * G < 148LL * kNrThreads) sh.chunk /= 2;
+    sh.cq = (a.num_q_heads + sh.chunk - 1) / sh.chunk;
+    sh.ck = (a.num_kv_heads + sh.chunk - 1) / sh.chunk;
+    sh.chunks = chunks(sh.chunk);
+    const int te = a.table_dtype == TT_DTYPE_F32 ? 4 : V;  // elements of a 16-byte load
+    sh.table_aligned = !(((uintptr_t)a.cos | (uintptr_t)a.sin) & 15) && a.cos_stride % te == 0 && a.sin_stride % te == 0;
+    sh.weight_aligned = !(((uintptr_t)a.q_weight | (uintptr_t)a.k_weight) & 15);
+    const long long threads = (long long)a.num_rows * sh.chunks * G;
+    const dim3 grid((unsigned)((threads + kNrBlock - 1) / kNrBlock)), block(kNrBlock);
+#define TT_NR(VV, SS, BB, FF) launch(k_norm_rope<T, TQ, TKV, VV, SS, BB, FF>, grid, block, 0, st, false, a, sh)
+    if (vec && steps == 1 && a.rot_dim == a.head_dim) return sh.chunk == 1 ? TT_NR(V, 1, 1, true) : TT_NR(V, 1, kNrBatch, true);
+    if (vec) return steps > 1 ? TT_NR(V, 2, 1, false) : TT_NR(V, 1, kNrBatch, false);
+    return steps <= 2 ? TT_NR(1, 2, 1, false) : TT_NR(1, 8, 1, false);
 #undef TT_NR
 }
 
@@ -498,10 +653,11 @@ tt_status tt_page_tables(const tt_page_tables_args* args, void* stream) {
     tt_status s = check_cuda(launch(k_page_scan<false>, dim3(1), dim3(kPtThreads), 0, st, false, a), "page_tables");
     if (s != TT_OK) return s;
     const int row_blocks = (int)(((long long)a.num_rows + kPrThreads * kPrRows - 1) / (kPrThreads * kPrRows));
+    const int wide = !(((uintptr_t)a.slots | (uintptr_t)a.positions | (uintptr_t)a.row_seq | (uintptr_t)a.row_lens) & 15);
     int seq_blocks = (a.num_seqs + kPrThreads / 32 - 1) / (kPrThreads / 32);
     seq_blocks = seq_blocks > 148 * 8 ? 148 * 8 : seq_blocks;
     return check_cuda(launch(k_page_rows, dim3((unsigned)(row_blocks + seq_blocks)), dim3(kPrThreads), 0, st, true, a,
-                             row_blocks), "page_tables");
+                             row_blocks, wide), "page_tables");
 }
 
 tt_status tt_qk_norm_rope(const tt_qk_norm_rope_args* args, void* stream) {
