@@ -16,12 +16,13 @@ from . import _C
 from ._lib import LIB_PATH
 from .cache import TriTierCache
 from .constants import CHUNK_SIZE, DEVICE, SINK_SIZE, UPDATE_THRESHOLD
+from .paged import SharedPrefixBatch
 
 __version__ = "0.1.0"
 
 HAS_CPP_EXT = True  # the compute path is the CUDA library; there is nothing else
 
-__all__ = ["TriTierCache", "DEVICE", "UPDATE_THRESHOLD", "CHUNK_SIZE", "SINK_SIZE", "HAS_CPP_EXT", "_C",
+__all__ = ["TriTierCache", "SharedPrefixBatch", "DEVICE", "UPDATE_THRESHOLD", "CHUNK_SIZE", "SINK_SIZE", "HAS_CPP_EXT", "_C",
            "__version__", "install_as_tri_tier", "LIB_PATH"]
 
 

@@ -15,6 +15,7 @@ from typing import Any, Dict, List, Optional, Tuple, Type
 
 import torch
 
+from .. import _C
 from ..cache import TriTierCache
 
 HAS_CPP_EXT = True
@@ -25,6 +26,9 @@ H_RATIO = 0.05
 SCORE_DECAY = 0.999
 K_GROUP_SIZE = 16
 PBS_METADATA_DTYPE = "fp16"
+# Decode steps: norm, rotation and the float32 rows of q, k and v in one kernel (qk_norm_rope) with one rounding
+# instead of the module's own steps in its dtype.  Set by apply_patch(fused_qk=True).
+FUSED_QK = False
 
 
 def _rotate_half(x: torch.Tensor) -> torch.Tensor:
@@ -53,6 +57,26 @@ def _reference_attention_path(self, cache: TriTierCache, Q: torch.Tensor, num_q_
     return torch.matmul(w, V_full).to(Q.device), w.to(Q.device)
 
 
+def _fused_rows(self, q, k, v, cos, sin, device):
+    """The float32 rows (Q, K, V) of one decode token by qk_norm_rope, or None where the module's norms or types
+    are not the kernel's."""
+    hd = q.shape[-1]
+    norms = [getattr(self, "q_norm", None), getattr(self, "k_norm", None)]
+    eps = {float(n.variance_epsilon) for n in norms if n is not None and hasattr(n, "variance_epsilon")}
+    if len(eps) > 1 or any(n is not None and not (hasattr(n, "variance_epsilon") and n.weight.shape == (hd,)) for n in norms):
+        return None
+    w = [None if n is None else n.weight.detach() for n in norms]
+    types = {t.dtype for t in w if t is not None}
+    if q.device != device or q.dtype not in (torch.float32, torch.bfloat16, torch.float16) or hd % 2 or hd > 512 or \
+            cos.shape[-1] != hd or cos.dtype not in (q.dtype, torch.float32) or len(types) > 1 or types - {q.dtype, torch.float32}:
+        return None
+    rows = [torch.empty((1, t.shape[2], hd), dtype=torch.float32, device=device) for t in (q, k, v)]
+    half = lambda t: t.detach().reshape(1, hd)[:, :hd // 2]  # noqa: E731
+    _C.qk_norm_rope(q.detach()[0], k.detach()[0], v.detach()[0], half(cos), half(sin), *rows, q_weight=w[0], k_weight=w[1],
+                    eps=eps.pop() if eps else 0.0)
+    return [t.view(-1) for t in rows]
+
+
 def patched_forward(self, hidden_states: torch.Tensor,
                     position_embeddings: Optional[Tuple[torch.Tensor, torch.Tensor]] = None,
                     attention_mask: Optional[torch.Tensor] = None, past_key_values: Optional[Any] = None,
@@ -77,6 +101,12 @@ def patched_forward(self, hidden_states: torch.Tensor,
     q = self.q_proj(hidden_states).view(bsz, q_len, nq, hd)
     k = self.k_proj(hidden_states).view(bsz, q_len, nkv, hd)
     v = self.v_proj(hidden_states).view(bsz, q_len, nkv, hd)
+    if FUSED_QK and q_len == 1 and not kwargs.get("output_attentions", False):
+        rows = _fused_rows(self, q, k, v, *position_embeddings, cache.device)
+        if rows is not None:
+            out = torch.empty(nq * hd, dtype=torch.float32, device=cache.device)
+            cache.step(*rows, out)
+            return self.o_proj(out.view(bsz, q_len, -1).to(dtype=hidden_states.dtype)), None
     if getattr(self, "q_norm", None) is not None:
         q = self.q_norm(q)
     if getattr(self, "k_norm", None) is not None:
@@ -130,9 +160,11 @@ for _mod, _cls in (("llama.modeling_llama", "LlamaAttention"), ("mistral.modelin
         pass
 
 
-def apply_patch():
-    """Patches every supported attention class (patch_model.py:209-216)."""
-    global _IS_PATCHED
+def apply_patch(fused_qk: bool = False):
+    """Patches every supported attention class (patch_model.py:209-216).  fused_qk: decode steps take q, k and v
+    through qk_norm_rope (no reference counterpart)."""
+    global _IS_PATCHED, FUSED_QK
+    FUSED_QK = bool(fused_qk)
     for cls in _SUPPORTED_ATTENTION_CLASSES:
         if cls not in _ORIGINAL_FORWARDS:
             _ORIGINAL_FORWARDS[cls] = cls.forward

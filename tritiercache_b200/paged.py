@@ -268,3 +268,71 @@ def shared_prefix_attention(q, k_pages, v_pages, prefix_table, prefix_len, table
     ws = torch.empty(size.value, dtype=torch.uint8, device=q.device) if size.value else None
     _run(L.tt_shared_prefix_attention, _PREFIX.pack(*first, 0 if ws is None else ws.data_ptr(), *rest), index,
          "shared_prefix_attention")
+
+
+class SharedPrefixBatch:
+    """A paged cache for requests that continue one shared prompt, and the
+    calls of a step over it::
+
+        batch = SharedPrefixBatch(num_pages, 16, num_kv_heads, head_dim, max_requests, max_pages, max_rows)
+        slots, positions = batch.set_prefix(n)      # then qk_norm_rope of the prompt's rows into these slots
+        batch.begin(new_lens)                       # pages, slots, positions of the step's rows
+        batch.place(q, k, v, cos, sin, q_out)       # norm, rotation, keys and values into the pages
+        batch.attend(q_out, out)                    # prompt once for all rows, then each row's own pages
+
+    The buffers belong to the object and keep their addresses, so a step can be
+    captured into a CUDA graph.  No reference counterpart.  ``max_rows`` is the
+    number of new tokens a step can hold; rows behind the step's are padding.
+    After ``begin``: ``lens`` [requests] tokens held, ``row_seq`` [rows] the
+    request of each row (-1: padding), ``deferred`` [1] the requests that found
+    no pages and wait.
+    """
+
+    def __init__(self, num_pages, page_size, num_kv_heads, head_dim, max_requests, max_pages, max_rows,
+                 dtype=torch.bfloat16, device=None):
+        if min(num_pages, page_size, num_kv_heads, head_dim, max_requests, max_pages, max_rows) <= 0:
+            raise ValueError("sizes must be positive.")
+        device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+        shape = (num_pages, page_size, num_kv_heads, head_dim)
+        self.k_pages, self.v_pages = (torch.zeros(shape, dtype=dtype, device=device) for _ in range(2))
+        new = lambda n, dt=_I32: torch.zeros(n, dtype=dt, device=device)  # noqa: E731
+        self.tables = torch.full((max_requests, max_pages), -1, dtype=_I32, device=device)
+        self.lens, self.cu_new, self.deferred = new(max_requests), new(max_requests + 1), new(1)
+        self.slots, self.positions, self.row_seq, self.row_lens = new(max_rows, _I64), new(max_rows), new(max_rows), new(max_rows)
+        self.free_pages = torch.arange(num_pages - 1, -1, -1, dtype=_I32, device=device)
+        self.free_count = torch.full((1,), num_pages, dtype=_I32, device=device)
+        self.page_size = page_size
+        self.prefix_len = 0
+        self.prefix_table = new(0)
+        self._num_pages, self._begun = num_pages, False
+
+    def set_prefix(self, length: int):
+        """Gives the shared prompt its pages (before the first step); returns the
+        slots and positions of its tokens."""
+        pages = -(-length // self.page_size)
+        if self._begun:
+            raise ValueError("the prefix is set before the first step.")
+        if length < 0 or pages > self._num_pages:
+            raise ValueError("the pool does not hold the prefix.")
+        dev = self.tables.device
+        self.prefix_len = length
+        self.prefix_table = torch.arange(pages, dtype=_I32, device=dev)  # the bottom of the stack is handed out last
+        self.free_pages.copy_(torch.arange(self._num_pages - 1, -1, -1, dtype=_I32, device=dev))
+        self.free_count.fill_(self._num_pages - pages)
+        t = torch.arange(length, device=dev)
+        return t, t.to(_I32)
+
+    def begin(self, new_lens) -> None:
+        """new_lens [requests] int32: new tokens, 0 rests, -1 has ended."""
+        page_tables(self.lens, new_lens, self.tables, self.free_pages, self.free_count, self.page_size, self.lens, self.cu_new,
+                    self.slots, self.positions, self.row_seq, self.row_lens, self.deferred, position_offset=self.prefix_len)
+        self._begun = True
+
+    def place(self, q, k, v, cos, sin, q_out, q_weight=None, k_weight=None, eps=1e-6) -> None:
+        """qk_norm_rope of the step's rows ([max_rows, heads, head_dim]) into the pages."""
+        qk_norm_rope(q, k, v, cos, sin, q_out, self.k_pages, self.v_pages, q_weight, k_weight, eps, self.positions, self.slots)
+
+    def attend(self, q, out, scale=None) -> None:
+        """shared_prefix_attention of the step's rows."""
+        shared_prefix_attention(q, self.k_pages, self.v_pages, self.prefix_table, self.prefix_len, self.tables, self.row_lens, out,
+                                row_seq=self.row_seq, scale=scale)
