@@ -640,3 +640,84 @@ def test_python_calls_refuse_what_does_not_fit(C_):
         with pytest.raises(ValueError):
             C_.page_tables(**{**ok, **bad})
     torch.cuda.synchronize()
+
+
+def test_numbers_that_do_not_fit_are_refused(C_):
+    s = make_attn(12, 3, 8, 2, 128, 40, [4, 5, 6], 16, BF)
+    i32 = lambda n: torch.zeros(n, device="cuda", dtype=torch.int32)  # noqa: E731
+    with pytest.raises(ValueError):
+        C_.shared_prefix_attention(s["q"], s["k"], s["v"], s["ptab"], 2 ** 40, s["tables"], s["lens"], torch.empty_like(s["q"]))
+    for kw in (dict(page_size=16.5), dict(page_size=2 ** 33), dict(position_offset=2 ** 31)):
+        with pytest.raises(ValueError):
+            C_.page_tables(i32(2), i32(2), torch.zeros((2, 4), device="cuda", dtype=torch.int32), i32(5), i32(1),
+                           seq_lens=i32(2), cu_new=i32(3), slots=i32(4).long(), positions=i32(4), row_seq=i32(4), row_lens=i32(4),
+                           deferred=i32(1), **{"page_size": 16, **kw})
+
+
+def test_attention_of_pools_with_shared_heads_and_single_pages(C_):
+    # the strides of dimensions of one entry say nothing, and heads may lie over one another (read only)
+    s = make_attn(13, 5, 8, 1, 128, 30, [1, 2, 3, 4, 5], 32, BF)
+    want = attend(C_, s)
+    one = {**s, "k": s["k"].as_strided(s["k"].shape, (*s["k"].stride()[:2], 3, 1)),
+           "v": s["v"].as_strided(s["v"].shape, (*s["v"].stride()[:2], 5, 1))}
+    assert torch.equal(attend(C_, one), want)
+    q = s["q"].repeat(1, 2, 1)
+    four = {**s, "q": q, "k": s["k"].expand(-1, -1, 2, -1), "v": s["v"].expand(-1, -1, 2, -1)}
+    got = attend(C_, four)
+    assert torch.equal(got[:, :8], want) and torch.equal(got[:, 8:], want)
+
+
+def test_attention_in_large_pools_and_pages(C_):
+    """Offsets beyond 32 bits: the pages in use lie at the end of a pool of over 2^32 bytes and 2^31 elements."""
+    P, nkv, hd, pages = 32768, 8, 128, 72
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("needs 20 GB of device memory")
+    k, v = (torch.empty((pages, P, nkv, hd), device="cuda", dtype=BF) for _ in range(2))
+    assert k.numel() > 2 ** 31
+    g = gen(14)
+    for p in (70, 71):
+        for x in (k, v):
+            x[p] = torch.randn((P, nkv, hd), generator=g, device="cuda").to(BF)
+    R = 6
+    s = dict(q=torch.randn((R, 16, hd), generator=g, device="cuda").to(BF), k=k, v=v,
+             ptab=torch.tensor([71], device="cuda", dtype=torch.int32), prefix=700,
+             tables=torch.full((R, 1), 70, device="cuda", dtype=torch.int32),
+             lens=torch.tensor([1, 40, 333, 1000, 7, 0], device="cuda", dtype=torch.int32),
+             seq=torch.arange(R, device="cuda", dtype=torch.int32), P=P)
+    attn_close(attend(C_, s), s, hd ** -0.5)
+    slots = torch.tensor([71 * P + 5, 70 * P + 9], device="cuda")
+    x = torch.randn((2, nkv, hd), generator=g, device="cuda").to(BF)
+    q = torch.zeros((2, 16, hd), device="cuda", dtype=BF)
+    C_.qk_norm_rope(q, x, x, None, None, q, k, v, slots=slots)
+    assert torch.equal(k.view(-1, nkv, hd)[slots], x) and torch.equal(v.view(-1, nkv, hd)[slots], x)
+
+
+def test_first_calls_may_be_captured(C_):
+    """In a process of their own: the first call of each operator is inside a stream capture."""
+    import subprocess
+    import sys
+    code = """
+import sys; sys.path[:0] = ['.', 'tests']
+import torch, test_gpu_paged as t
+from tritiercache_b200 import _C
+s = t.make_attn(1, 9, 8, 2, 128, 300, [3] * 9, 16, torch.bfloat16)
+q = torch.zeros_like(s['q']); k = torch.zeros((9, 2, 128), device='cuda', dtype=torch.bfloat16)
+out = torch.zeros_like(q)
+i32 = lambda n: torch.zeros(n, device='cuda', dtype=torch.int32)
+a = [i32(2), i32(2), torch.zeros((2, 4), device='cuda', dtype=torch.int32), i32(5), i32(1), 16, i32(2), i32(3), i32(9000).long(),
+     i32(9000), i32(9000), i32(9000), i32(1)]
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    _C.qk_norm_rope(q, k, k, None, None, q, k, k)
+    _C.page_tables(*a)
+    t.attend(_C, s, out=out)
+g.replay()
+torch.cuda.synchronize()
+assert torch.equal(out, t.attend(_C, s)) and int(a[8][0]) == -1
+print('captured')
+"""
+    import os
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=root, timeout=300)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]

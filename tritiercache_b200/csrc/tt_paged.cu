@@ -156,15 +156,24 @@ __global__ void __launch_bounds__(kPtThreads) k_page_scan(const tt_page_tables_a
                 p.cu_new[b] = clamp_i32(at.b);
                 if (SMALL) cu_s[b] = clamp_i32(at.b);
             }
-            // the warp copies the pages of each of its ended requests together
+            // the warp copies the pages of its ended requests, four requests at a time, eight lanes each (their
+            // table rows are not written in this call)
             unsigned todo = __ballot_sync(~0u, back[i] > 0);
             while (todo) {
-                const int l = __ffs(todo) - 1;
-                todo &= todo - 1;
+                unsigned rest = todo;
+                for (int k = (tid & 31) >> 3; k && rest; --k) rest &= rest - 1;
+                const int l = rest ? __ffs(rest) - 1 : 0;
                 const int bb = base + ((tid & ~31) + l) * kPtItems + i, cnt = __shfl_sync(~0u, back[i], l);
                 const long long dst = __shfl_sync(~0u, at.a, l);
-                for (int j = tid & 31; j < cnt; j += 32)
-                    if (dst + j < p.free_capacity) p.free_pages[dst + j] = p.tables[bb * p.table_stride + j];
+                const int32_t* row = p.tables + bb * p.table_stride;
+                if (rest) {
+#pragma unroll 4
+                    for (int j = tid & 7; j < cnt; j += 8) {
+                        const int page = __ldg(row + j);
+                        if (dst + j < p.free_capacity) p.free_pages[dst + j] = page;
+                    }
+                }
+                for (int k = 0; k < 4; ++k) todo &= todo - 1;
             }
             at.a += back[i];
             at.b += r[i].n;

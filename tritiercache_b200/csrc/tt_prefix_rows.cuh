@@ -1,5 +1,5 @@
-// tt_prefix_rows.cuh -- the pass of tt_shared_prefix_attention over each row's own pages, which also
-// joins what the prefix pass left.
+// tt_prefix_rows.cuh -- the pass of tt_shared_prefix_attention over each row's own pages, and the join of
+// both passes.
 //
 // `splits` CTAs per (row, kv head, tile of up to 8*NB query heads).  Their 4*splits warps take the row's
 // tokens in groups of 16 (a group never crosses a page), warp w groups w, w+4*splits, ...; each warp keeps its
@@ -16,7 +16,12 @@
 // CTAs joining the prefix pass's partials themselves, cost more: the CTAs wait for the prefix pass, where they
 // could run beside it, its time being the tensor cores' and theirs the memory's.)
 //
-// Bound: HBM (the row's K and V are read once, by one cluster).
+// Loads are TMA boxes of 16 tokens (cp.async by the lanes instead cost the warps a third of their instructions,
+// and beside the prefix pass more: 282 against 257 us for 256 rows on 32k).  Weights are rounded to the pages'
+// type for the second product, as in the prefix pass; logits, exponentials and sums are float32.
+//
+// Bound: HBM (each row's K and V are read once).  Alone, 256 rows of up to 2048 tokens (1.08 GB): 170 us,
+// 6.3 TB/s.
 #pragma once
 #include <cuda.h>
 #include <cuda_bf16.h>

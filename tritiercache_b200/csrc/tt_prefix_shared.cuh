@@ -20,6 +20,15 @@
 // Warps: 0 loads K and V (TMA, one box per page and 64 channels, 128-byte swizzle), 1 issues the matrix
 // instructions, 2 clears the V rows behind the prefix's end (what lies there may be NaN, and 0 * NaN is not
 // 0), 4-7 and 8-11 are the softmax of the two accumulators and load their queries.
+//
+// Bound: 256 rows of 32 heads on 32k take 144 us (950 TFLOP/s; 83 us at the measured GEMM rate), 2.5 us a key
+// tile of 256 rows.  Neither the exponentials (16 a clock: half of that), nor the products alone, nor the loads
+// set it: removing any one gains under a tenth.  It is the chain S -> weights -> products through barriers, with
+// the two softmax warps that share a scheduler with the warp issuing the products slower than the others by
+// half.  Measured beside it and no faster: the tile as a pair of CTAs (cta_group::2; 161 us, the arrivals
+// between the CTAs cost more than the shared K and V save), steps of 64 keys with two S an accumulator
+// (146-168 us; a product of 64 columns takes as long as one of 128), a quarter of the exponentials as
+// polynomials (139 against 143), five K/V slots (143 us, but no rows' CTA beside them).
 #pragma once
 #include "tt_prefix_rows.cuh"
 
