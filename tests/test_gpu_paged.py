@@ -721,3 +721,104 @@ print('captured')
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=root, timeout=300)
     assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
+
+
+# ---------------------------------------------------------------------------------------------
+# attention at sizes where the shared prefix has a pass of its own
+# ---------------------------------------------------------------------------------------------
+SHARED = [
+    # R, nq, nkv, hd, prefix, longest own, page, type, rows a request, layout
+    (70, 8, 8, 128, 127, 20, 16, BF, 1, "nhd"),      # one head a kv head, a prefix short of a tile
+    (66, 16, 8, 128, 128, 20, 32, F16, 1, "hnd"),
+    (65, 8, 8, 128, 129, 40, 16, BF, 1, "kv"),       # a tile of one key
+    (300, 16, 2, 128, 130, 10, 64, F16, 3, "nhd"),   # 2400 rows of heads a kv head: ten row tiles
+    (33, 24, 8, 128, 1000, 50, 128, BF, 1, "hnd"),   # 99 rows of heads: even and odd key tiles
+    (16, 64, 8, 128, 1024, 30, 256, F16, 1, "nhd"),  # 128 rows of heads exactly
+    (17, 64, 8, 128, 1025, 30, 32, BF, 1, "nhd"),    # 136: the second half almost empty
+    (90, 6, 3, 64, 777, 60, 16, F16, 2, "kv"),
+    (200, 12, 1, 64, 999, 30, 16, BF, 1, "nhd"),     # 12 heads: two tiles of 8 in the rows' pass
+    (40, 34, 2, 128, 2000, 20, 16, BF, 1, "nhd"),    # 17 heads a kv head
+    (512, 4, 1, 64, 513, 3, 16, BF, 1, "nhd"),       # 2048 rows, one kv head
+    (3, 128, 16, 128, 4097, 100, 16, F16, 1, "nhd"), # few rows, spans across kv heads
+    (24, 32, 8, 128, 6000, 300, 64, BF, 1, "hnd"),
+]
+
+
+@pytest.mark.parametrize("R,nq,nkv,hd,prefix,most,P,dt,chunk,layout", SHARED)
+def test_shared_pass_matches_the_formula(C_, R, nq, nkv, hd, prefix, most, P, dt, chunk, layout):
+    r = np.random.default_rng(R + prefix)
+    lens = r.integers(0, most + 1, R)
+    lens[0] = most
+    if R > 3:
+        lens[1], lens[2] = 0, 1
+    s = make_attn(R + hd, R, nq, nkv, hd, prefix, lens, P, dt, chunk, layout)
+    poison_tail(s)
+    attn_close(attend(C_, s), s, hd ** -0.5)
+
+
+@pytest.mark.parametrize("R,nq,hd", [(40, 16, 128), (20, 16, 128), (80, 16, 64)])
+def test_shared_pass_with_rising_maxima_padding_and_in_place(C_, R, nq, hd):
+    for dt in (BF, F16):
+        s = make_attn(31, R, nq, 4, hd, 1500, np.arange(R) % 50, 16, dt)
+        s["k"] *= (torch.arange(1, s["k"].shape[0] + 1, device="cuda").to(dt) / 16)[:, None, None, None]
+        attn_close(attend(C_, s, scale=0.3), s, 0.3)
+        s["q"][5] = float("nan")
+        s["seq"][5] = -1
+        out = attend(C_, s)
+        live = [r for r in range(R) if r != 5]
+        keep = {k: (v[live] if k in ("q", "lens", "seq") else v) for k, v in s.items()}
+        attn_close(out[live], keep, hd ** -0.5)
+        assert bool((out[5] == 5).all())
+        again = attend(C_, s)
+        assert torch.equal(again, out)
+        s["q"][5] = 5.0
+        attend(C_, s, out=s["q"])
+        assert torch.equal(s["q"], out)
+
+
+@pytest.mark.parametrize("R", [24, 90])
+def test_shared_pass_bad_pages_nan_and_infinity(C_, R):
+    s = make_attn(32, R, 16, 4, 128, 1333, np.full(R, 50), 16, BF)
+    good = attend(C_, s)
+    attn_close(good, s, 128 ** -0.5)
+    s["tables"][1, 2] = s["k"].shape[0]
+    s["lens"][3] = s["tables"].shape[1] * 16 + 1
+    out = attend(C_, s)
+    assert bool(torch.isnan(out[[1, 3]]).all())
+    rest = [r for r in range(R) if r not in (1, 3)]
+    assert torch.equal(out[rest], good[rest])
+    keep = s["ptab"].clone()
+    for bad in (-1, s["k"].shape[0], 1 << 30):
+        for at in (0, 40, len(keep) - 1):
+            s["ptab"].copy_(keep)
+            s["ptab"][at] = bad
+            assert bool(torch.isnan(attend(C_, s)).all())
+    s["ptab"].copy_(keep)
+    page = s["ptab"][50].long()
+    s["v"][page, 3, 2] = float("inf")   # a value of kv head 2: its heads alone
+    s["k"][s["ptab"][60].long(), 1, 0] = float("nan")
+    out = attend(C_, s)
+    assert bool(torch.isnan(out[rest][:, :4]).all()) and bool((~torch.isfinite(out[rest][:, 8:12])).all())
+    assert torch.equal(out[rest][:, 4:8], good[rest][:, 4:8]) and torch.equal(out[rest][:, 12:], good[rest][:, 12:])
+
+
+def test_shared_pass_queries_that_16_byte_loads_do_not_fit(C_):
+    s = make_attn(33, 40, 16, 4, 128, 1200, np.full(40, 9), 16, F16)
+    ref = attend(C_, s)
+    wide = torch.zeros((40, 17, 130), device="cuda", dtype=F16)
+    wide[:, 1:, 2:] = s["q"]
+    assert torch.equal(attend(C_, {**s, "q": wide[:, 1:, 2:]}, out=torch.empty_like(s["q"])), ref)
+
+
+def test_shared_pass_in_two_streams_at_once(C_):
+    cases = [make_attn(40 + i, 64, 32, 8, (128, 64)[i % 2], 3000, np.full(64, 200), 32, (BF, F16)[i // 2]) for i in range(4)]
+    want = [attend(C_, s) for s in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    got = [[torch.zeros_like(w) for _ in range(6)] for w in want]
+    for i in range(6):
+        for s, st, o in zip(cases, streams, got):
+            with torch.cuda.stream(st):
+                attend(C_, s, out=o[i])
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, w) for os, w in zip(got, want) for o in os)

@@ -11,6 +11,7 @@ namespace tt {
 static_assert(sizeof(tt_shared_prefix_args) == 208, "packed by paged.py");
 
 constexpr int kSms = 148;
+constexpr long long kWalk = 1 << 23;
 constexpr int kCross = 4;  // measured: 7 tiles in 30 us, 7 in two spans in 40 (384 rows of heads on 8k)
 
 // All kernels ask for the whole of an SM's shared memory: the passes' CTAs share one, and an SM that has to
@@ -118,9 +119,12 @@ static PrefixParams plan_prefix(const tt_shared_prefix_args& a) {
     p.group = a.num_q_heads / a.num_kv_heads;
     while ((1 << p.page_shift) < a.page_size) ++p.page_shift;
     p.head_tiles = p.group <= 8 ? 1 : (p.group + 15) / 16;
-    // One row has nobody to share with.  The prefix pass takes its maxima before the scale, so the scale must
-    // not turn them round.
-    p.walk_prefix = a.num_rows < 2 || a.prefix_len == 0 || !(a.scale > 0.f);
+    // One row has nobody to share with, and reading a short prefix again for each of a few rows, from L2, costs less
+    // than a pass of its own and its partials (32/8 heads of 128: 8 rows on 512 tokens 9.5 against 12.5 us, on 1024
+    // 11.5 against 12.7, on 2048 15.2 against 13.0; 2 rows on 4096 11.4 against 12.6; 16 rows on 512 10.9 against 14.0).
+    // The prefix pass takes its maxima before the scale, so the scale must not turn them round.
+    const long long again = (long long)a.num_rows * a.prefix_len * a.num_kv_heads * p.head_tiles * a.head_dim;
+    p.walk_prefix = a.num_rows < 2 || again <= kWalk || !(a.scale > 0.f);
     if (!p.walk_prefix) {
         const int rows = a.num_rows * p.group;
         p.tile_rows = rows > kPsTile ? 2 * kPsTile : kPsTile;
