@@ -822,3 +822,18 @@ def test_shared_pass_in_two_streams_at_once(C_):
                 attend(C_, s, out=o[i])
     torch.cuda.synchronize()
     assert all(torch.equal(o, w) for os, w in zip(got, want) for o in os)
+
+
+def test_attention_without_tables_of_its_own(C_):
+    for R in (1, 3, 60):
+        s = make_attn(50, R, 16, 4, 128, 900, np.zeros(R, np.int32), 16, BF)
+        want = attend(C_, s)
+        attn_close(want, s, 128 ** -0.5)
+        none = {**s, "tables": torch.zeros((R, 0), device="cuda", dtype=torch.int32)}  # tables of no pages
+        assert torch.equal(attend(C_, none), want)
+        none["lens"] = torch.ones_like(s["lens"])  # a token that no table has
+        assert bool(torch.isnan(attend(C_, none)).all())
+        pad = {**s, "tables": torch.zeros((0, 4), device="cuda", dtype=torch.int32), "seq": torch.full_like(s["seq"], -1)}
+        assert bool((attend(C_, pad) == 5).all())  # nothing but padding
+        empty = {**s, "prefix": 0, "ptab": None}
+        assert bool((attend(C_, empty) == 0).all())
