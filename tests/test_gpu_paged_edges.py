@@ -1,0 +1,29 @@
+"""The paged operators at the edges of their arguments' ranges."""
+import numpy as np
+import pytest
+import torch
+
+from test_gpu_paged import C_, same, tables_gpu, tables_ref  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+TOP = 2 ** 31 - 1
+
+
+@pytest.mark.parametrize("B", [9, 2500])  # one launch, two launches
+@pytest.mark.parametrize("P", [1, 2, 16])
+def test_page_tables_lengths_at_the_top_of_their_type(C_, B, P):  # noqa: F811
+    """A request that claims up to 2^31 - 1 tokens and brings more is deferred (with pages of one token the sum needs
+    more than 31 bits of pages), its neighbours get theirs."""
+    W = 3
+    ctx, new = np.zeros(B, np.int32), np.ones(B, np.int32)
+    ctx[:7] = [TOP, TOP - 1, 1, TOP, TOP, 2, TOP]
+    new[:7] = [1, 1, 1, 7, 0, 1, -1]
+    tables = np.arange(B * W, dtype=np.int32).reshape(B, W)
+    free = np.arange(B * W, 2 * B * W + 20, dtype=np.int32)
+    rows = int(np.maximum(new, 0).sum()) + 3
+    count = len(free) - 10
+    want = tables_ref(ctx, new, tables, free, count, P, rows, 0)
+    assert want["deferred"][0] == 3
+    same(tables_gpu(C_, ctx, new, tables, free, count, P, rows, 0), want)
+    same(tables_gpu(C_, ctx, new, tables, free, count, P, rows, 0, in_place=True), want)

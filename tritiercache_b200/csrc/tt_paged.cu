@@ -64,10 +64,10 @@ __device__ __forceinline__ Pair64 block_scan2(Pair64 v, Pair64* tot, Pair64* sm)
 
 __device__ __forceinline__ int clamp_i32(long long x) { return x > INT_MAX ? INT_MAX : (int)x; }
 
-// Pages that hold x tokens (x below 2^32).
-__device__ __forceinline__ int pt_pages(const tt_page_tables_args& p, long long x) {
+// Pages that hold x tokens (x below 2^32: so may be the pages, where a page is one token).
+__device__ __forceinline__ long long pt_pages(const tt_page_tables_args& p, long long x) {
     const uint32_t u = (uint32_t)x, P = (uint32_t)p.page_size;
-    return (int)(u / P) + (u % P != 0);
+    return (long long)(u / P) + (u % P != 0);
 }
 
 struct PtReq {
@@ -94,7 +94,7 @@ struct PtRow {
 __device__ __forceinline__ PtRow pt_row(const tt_page_tables_args& p, int b, int ctx, int cu, int first, int top,
                                         int t) {
     if (first < 0) return PtRow{-1, 0, -1, 0};
-    const int held = pt_pages(p, ctx);
+    const int held = (int)pt_pages(p, ctx);
     const int pos = ctx + (t - cu), pg = pos / p.page_size;
     const int page = pg < held ? p.tables[b * p.table_stride + pg] : p.free_pages[top - 1 - first - (pg - held)];
     return PtRow{(long long)page * p.page_size + pos % p.page_size, pos + p.position_offset, b, pos + 1};
@@ -294,7 +294,7 @@ __global__ void __launch_bounds__(kPrThreads) k_page_rows(const tt_page_tables_a
         for (int b = w; b < B; b += nw) {
             const int n = p.new_lens[b];
             if (first[b] < 0 || n <= 0) continue;
-            const int held = pt_pages(p, ctx[b]), given = pt_pages(p, (long long)ctx[b] + n) - held;
+            const int held = (int)pt_pages(p, ctx[b]), given = (int)(pt_pages(p, (long long)ctx[b] + n) - held);
             for (int j = lane; j < given; j += 32)
                 p.tables[b * p.table_stride + held + j] = p.free_pages[top - 1 - first[b] - j];
         }
