@@ -164,7 +164,7 @@ k_prefix_shared(const PrefixParams p, const __grid_constant__ CUtensorMap kmap, 
             bar_init(full + 8 * i, 1);
             bar_init(empty + 8 * i, 1);
         }
-        bar_init(q_full, PAIR ? 256 : 128);
+        bar_init(q_full, 256);
         for (int t = 0; t < 2; ++t) {
             bar_init(s_full + 8 * t, 1);
             bar_init(p_ready + 16 * t, 128);
@@ -328,7 +328,7 @@ k_prefix_shared(const PrefixParams p, const __grid_constant__ CUtensorMap kmap, 
         const uint32_t lanes = tmem + ((uint32_t)(row & 96) << 16), s_col = lanes + t * 128, o_col = lanes + S::kTmemO + t * HD;
         const int rows_all = a.num_rows * p.group;
         const bool q16 = !(((uintptr_t)a.q & 15) | ((a.q_row_stride | a.q_head_stride) & 7));
-        uint32_t phase = 0;
+        uint32_t phase = 0, q_phase = 0;
         ps_spans(p, [&](int kvh, int tile, long long slot_at, int k0, int n) {
             const int mine = PAIR ? n : (n - t + 1) / 2;
             const int mrow = tile * p.tile_rows + (PAIR ? t * kPsTile : 0) + row;
@@ -351,8 +351,14 @@ k_prefix_shared(const PrefixParams p, const __grid_constant__ CUtensorMap kmap, 
                     *reinterpret_cast<uint4*>(dst + (c / 8) * S::kHalf + (((c % 8) ^ (row & 7)) << 4)) = x;
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                bar_arrive(q_full);
             }
+            // Accumulator 1 of !PAIR has loaded nothing, but arrives too: it has seen the last O_1 of the span before.
+            // Without that s_full[1] could complete twice before a late warp looks once, and the warp would wait for a
+            // phase that itself waits for the warp.  With no tile in this span it waits for the others' arrivals, lest
+            // it arrive twice in one phase.
+            bar_arrive(q_full);
+            if (!PAIR && mine == 0 && !bar_wait_warp(q_full, q_phase, abort)) return false;
+            q_phase ^= 1;
             float m = -INFINITY, l = 0.f;
             for (int i = 0; i < mine; ++i) {
                 if (!bar_wait_warp(s_full + 8 * t, phase, abort)) return false;
