@@ -15,17 +15,18 @@ CROSSING = [
     # rows of heads in one tile of 128: even and odd key tiles
     (8, 96, 96, 128, 2000, 30, 16, BF, 1, "nhd"),
     (8, 96, 96, 64, 2049, 30, 32, F16, 1, "kv"),      # a last key tile of one key
-    (20, 100, 50, 128, 1793, 9, 16, F16, 2, "hnd"),   # 15 key tiles
+    (20, 100, 50, 128, 3841, 9, 16, F16, 2, "hnd"),   # 31 key tiles
     (100, 40, 40, 128, 16385, 40, 64, BF, 1, "nhd"),
     (32, 32, 32, 128, 32769, 20, 128, F16, 1, "nhd"),
-    (64, 37, 37, 64, 16700, 33, 16, BF, 1, "hnd"),
+    (64, 40, 40, 64, 16700, 33, 16, BF, 1, "hnd"),
     (40, 149, 149, 64, 1281, 9, 16, BF, 1, "nhd"),    # more kv heads than CTAs: spans over whole ones
+    (40, 300, 300, 64, 600, 9, 16, F16, 1, "nhd"),    # spans of one key tile among them
     # tiles of 256
     (130, 96, 96, 128, 1999, 20, 16, F16, 1, "nhd"),
     (256, 32, 8, 128, 16400, 30, 32, BF, 1, "nhd"),
-    (140, 50, 50, 64, 3001, 20, 16, BF, 1, "kv"),
+    (140, 96, 96, 64, 3001, 20, 16, BF, 1, "kv"),
     # several row tiles of a kv head: side by side, and one after the other
-    (300, 48, 48, 128, 1700, 10, 16, BF, 1, "nhd"),
+    (300, 48, 48, 128, 1999, 10, 16, BF, 1, "nhd"),
     (600, 16, 2, 128, 9001, 10, 32, F16, 1, "nhd"),   # 19 row tiles
     (600, 16, 2, 64, 9100, 10, 16, BF, 3, "hnd"),
 ]

@@ -10,10 +10,6 @@ namespace tt {
 
 static_assert(sizeof(tt_shared_prefix_args) == 208, "packed by paged.py");
 
-constexpr int kSms = 148;
-constexpr long long kWalk = 1 << 23;
-constexpr int kCross = 4;  // measured: 7 tiles in 30 us, 7 in two spans in 40 (384 rows of heads on 8k)
-
 // All kernels ask for the whole of an SM's shared memory: the passes' CTAs share one, and an SM that has to
 // divide its memory anew between two kernels has to run dry first.  Once per kernel and device.
 template <auto Kern>
@@ -102,62 +98,6 @@ static tt_status check_prefix(const tt_shared_prefix_args* args) {
     if (((uintptr_t)a.k & 15) || ((uintptr_t)a.v & 15) || ((uintptr_t)a.q & 3))
         return set_error(TT_ERR_UNSUPPORTED, "shared_prefix_attention: k and v must be 16-byte aligned, q 4-byte aligned.");
     return TT_OK;
-}
-
-static int prefix_groups(const PrefixParams& p) {
-    return p.spans ? p.units * p.spans : (int)(((long long)p.units * p.kv_tiles + p.per - 1) / p.per);
-}
-static size_t prefix_slots(const PrefixParams& p) {
-    return p.walk_prefix ? 0 : 2 * ((size_t)prefix_groups(p) + (size_t)p.units) * p.lanes;
-}
-static size_t own_slots(const PrefixParams& p) { return p.join ? (size_t)p.splits * p.a.num_rows * p.a.num_q_heads : 0; }
-
-static PrefixParams plan_prefix(const tt_shared_prefix_args& a) {
-    PrefixParams p = {};
-    p.a = a;
-    p.scale_log2 = a.scale * 1.4426950408889634f;
-    p.group = a.num_q_heads / a.num_kv_heads;
-    while ((1 << p.page_shift) < a.page_size) ++p.page_shift;
-    p.head_tiles = p.group <= 8 ? 1 : (p.group + 15) / 16;
-    // One row has nobody to share with, and reading a short prefix again for each of a few rows, from L2, costs less
-    // than a pass of its own and its partials (32/8 heads of 128: 8 rows on 512 tokens 9.5 against 12.5 us, on 1024
-    // 11.5 against 12.7, on 2048 15.2 against 13.0; 2 rows on 4096 11.4 against 12.6; 16 rows on 512 10.9 against 14.0).
-    // The prefix pass takes its maxima before the scale, so the scale must not turn them round.
-    const long long again = (long long)a.num_rows * a.prefix_len * a.num_kv_heads * p.head_tiles * a.head_dim;
-    p.walk_prefix = a.num_rows < 2 || again <= kWalk || !(a.scale > 0.f);
-    if (!p.walk_prefix) {
-        const int rows = a.num_rows * p.group;
-        p.tile_rows = rows > kPsTile ? 2 * kPsTile : kPsTile;
-        p.row_tiles = (rows + p.tile_rows - 1) / p.tile_rows;
-        p.kv_tiles = (a.prefix_len + kPsTile - 1) / kPsTile;
-        // CTA groups over all row tiles of a kv head, unless they would leave more than a tenth of the SMs idle
-        p.lanes = kSms / p.row_tiles * p.row_tiles * 10 >= kSms * 9 ? p.row_tiles : 1;
-        p.units = a.num_kv_heads * (p.row_tiles / p.lanes);
-        const int groups = kSms / p.lanes;
-        // Equal spans across units use every SM, but a CTA whose span crosses a unit's border starts and ends twice,
-        // which costs it about kCross key tiles; whole spans per unit may leave SMs idle.
-        p.per = (int)(((long long)p.units * p.kv_tiles + groups - 1) / groups);
-        if (p.units <= groups) {
-            const int whole = (p.kv_tiles + groups / p.units - 1) / (groups / p.units);
-            if (whole <= p.per + kCross) p.per = whole, p.spans = 1;
-        }
-        // A span of one key tile leaves as many bytes of partials as two, and a 128-row tile's second accumulator
-        // without work (64 rows of 32 heads on 2k: 27.8 -> 23.2 us; at least four tiles: 25.5).
-        if (p.per < 2) p.per = 2;
-        if (p.spans) p.spans = (p.kv_tiles + p.per - 1) / p.per;
-    }
-    // CTAs of the rows' pass per row and head tile: two for each SM in all, if that leaves a warp two groups
-    const long long tokens = (long long)a.table_width * a.page_size + (p.walk_prefix ? a.prefix_len : 0);
-    const long long units = (long long)a.num_rows * a.num_kv_heads * p.head_tiles;
-    const long long most = tokens / (kRowWarps * kGroup * 2), fit = 2 * kSms / units;
-    p.splits = (int)(most < fit ? most : fit);
-    if (p.splits < 1) p.splits = 1;
-    p.join = p.splits > 1 || !p.walk_prefix;
-    return p;
-}
-
-static size_t prefix_workspace(const PrefixParams& p) {
-    return (prefix_slots(p) * kPsTile + own_slots(p)) * (p.a.head_dim * sizeof(float) + sizeof(float2));
 }
 
 // The pool in boxes of 64 channels and `tokens` tokens of one head.

@@ -28,37 +28,15 @@
 
 #include "tt_common.cuh"
 #include "tt_launch.cuh"
+#include "tt_prefix_plan.cuh"
 
 namespace tt {
 
 constexpr float kSlack = 8.f;    // log2 units a logit may exceed the reference before it is raised
-constexpr int kRowWarps = 4;
-constexpr int kGroup = 16;       // tokens per warp step
 
 constexpr long long kPatience = 4000000000LL;  // clocks that a wait may take (about two seconds)
 
 __device__ int g_prefix_error = 0;  // a wait that ran out (TT_ERR_TIMEOUT); reported by tt_device_error
-
-struct PrefixParams {
-    tt_shared_prefix_args a;
-    float scale_log2;            // scale * log2(e)
-    int page_shift;
-    int group;                   // query heads per kv head
-    int head_tiles;              // tiles of 8*NB query heads per kv head
-    int splits;                  // CTAs per row and head tile in the rows' pass
-    // prefix pass: a unit is a kv head and one tile of tile_rows rows of its (row, head of the group) matrix, or
-    // with lanes = row_tiles all its tiles at once, one CTA of a group of `lanes` each.  The flattened (unit, key
-    // tile) list is cut into spans of `per` for the groups: `spans` a unit, or, with spans = 0, across units.
-    // A span's partials are in slots 2 ((group + unit) lanes + lane) + t of 128 rows: t is the half of a 256-row
-    // tile, or even and odd key tiles of a 128-row one
-    int walk_prefix;             // 1: no prefix pass, the rows' pass reads the prefix too
-    int tile_rows, row_tiles, lanes, units, kv_tiles, per, spans;
-    float* part_o;               // [slot][128][hd]
-    float2* part_ml;             // [slot][128] (m in log2 units, l)
-    int join;                    // 1: the rows' pass leaves partials [splits][num_rows][num_q_heads] for k_prefix_join; 0: outputs
-    float* own_o;
-    float2* own_ml;
-};
 
 template <typename T> __device__ __forceinline__ void mma16816(float* c, const uint32_t* a, uint32_t b0, uint32_t b1);
 template <>
@@ -217,32 +195,18 @@ __global__ void __launch_bounds__(kJoinWarps * 32) k_prefix_join(const PrefixPar
     const long long rh = (long long)blockIdx.x * (kJoinWarps / W) + warp / W, all = (long long)a.num_rows * a.num_q_heads;
     const int r = (int)(rh / a.num_q_heads), head = (int)(rh % a.num_q_heads);
     const bool on = rh < all && !(a.row_seq && a.row_seq[r] < 0);
-    // the prefix pass's partials of this row: np of them, `step` slots of 128 rows apart from `first`
-    long long first = 0, step = 0;
-    int np = 0;
-    if (!p.walk_prefix) {
-        const int kvh = head / p.group, row = r * p.group + head % p.group;
-        const int tile = row / p.tile_rows, in = row % p.tile_rows, lane = p.lanes > 1 ? tile : 0;
-        const bool pair = p.tile_rows == 256;
-        const int u = p.lanes > 1 ? kvh : kvh * p.row_tiles + tile;
-        const int g0 = p.spans ? u * p.spans : u * p.kv_tiles / p.per;
-        const int g1 = p.spans ? g0 + p.spans - 1 : ((u + 1) * p.kv_tiles - 1) / p.per;
-        // even and odd key tiles are neighbours (!pair has one row tile, so one lane)
-        first = (2 * ((long long)(g0 + u) * p.lanes + lane) + (pair ? in >> 7 : 0)) * 128 + (in & 127);
-        step = (pair ? 2 * p.lanes : 1) * 128;
-        np = (g1 - g0 + 1) * (pair ? 1 : 2);
-    }
-    const int n = on ? (p.splits + np - sub + W - 1) / W : 0;
+    const PrefixPartials pre = on && !p.walk_prefix ? prefix_partials(p, r, head) : PrefixPartials{0, 0, 0};
+    const int n = on ? (p.splits + pre.n - sub + W - 1) / W : 0;
     pdl_wait();
     float M, L, acc[HD / 32];
     join_partials<HD>(n,
                       [&](int k) {
                           const int i = k * W + sub;
-                          return *(i < p.splits ? p.own_ml + (i * all + rh) : p.part_ml + (first + (i - p.splits) * step));
+                          return *(i < p.splits ? p.own_ml + (i * all + rh) : p.part_ml + (pre.first + (i - p.splits) * pre.step));
                       },
                       [&](int k) {
                           const int i = k * W + sub;
-                          return i < p.splits ? p.own_o + (i * all + rh) * HD : p.part_o + (first + (i - p.splits) * step) * HD;
+                          return i < p.splits ? p.own_o + (i * all + rh) * HD : p.part_o + (pre.first + (i - p.splits) * pre.step) * HD;
                       },
                       M, L, acc);
     if constexpr (W > 1) {

@@ -35,7 +35,6 @@
 namespace tt {
 
 constexpr int kPsThreads = 384;
-constexpr int kPsTile = 128;                       // keys per tile, rows per accumulator
 
 template <int HD, bool PAIR> struct PsShape {
     static constexpr int kSlot = kPsTile * HD * 2;                 // a K or V tile
@@ -121,27 +120,10 @@ template <typename T> constexpr uint32_t ps_idesc(int n, bool b_mn) {
     return 1u << 4 | fmt << 7 | fmt << 10 | (b_mn ? 1u << 16 : 0u) | (uint32_t)(n >> 3) << 17 | (uint32_t)(kPsTile >> 4) << 24;
 }
 
-// The spans of this CTA: fn(kv head, row tile, slot, first key tile, key tiles) for each, until fn returns false.
-// p.spans > 0: so many spans a unit, none crosses units; else the flattened list in spans of p.per.
+// The spans of this CTA.
 template <typename F>
 __device__ __forceinline__ void ps_spans(const PrefixParams& p, F fn) {
-    const int group = blockIdx.x / p.lanes, lane = blockIdx.x % p.lanes;
-    long long f, end;
-    if (p.spans) {
-        const long long u = group / p.spans;
-        f = u * p.kv_tiles + (long long)(group % p.spans) * p.per;
-        end = min(f + p.per, (u + 1) * p.kv_tiles);
-    } else {
-        f = (long long)group * p.per;
-        end = min(f + p.per, (long long)p.units * p.kv_tiles);
-    }
-    while (f < end) {
-        const int u = (int)(f / p.kv_tiles), k0 = (int)(f % p.kv_tiles);
-        const int n = (int)min(end - f, (long long)(p.kv_tiles - k0));
-        const int kvh = p.lanes > 1 ? u : u / p.row_tiles, tile = p.lanes > 1 ? lane : u % p.row_tiles;
-        if (!fn(kvh, tile, (long long)(group + u) * p.lanes + lane, k0, n)) return;
-        f += n;
-    }
+    prefix_spans(p, blockIdx.x / p.lanes, blockIdx.x % p.lanes, fn);
 }
 
 template <typename T, int HD, bool PAIR>
