@@ -497,9 +497,10 @@ tt_status tt_qk_norm_rope(const tt_qk_norm_rope_args* args, void* stream);
  * k and v: pools of num_pages pages, element (page, token, head, channel) at
  * page * page_stride + token * token_stride + head * head_stride + channel, all
  * strides multiples of 8 elements, bases 16-byte aligned.  page_size: a power of
- * two from 16 to 32768.  head_dim 64 or 128.  dtype (q, k, v, out): bf16 or f16; scores,
- * softmax and sums are float32, the weights are rounded to dtype for the second
- * product.  q and out have row and head strides in elements (multiples of 2 for q); out
+ * two from 16 to 32768.  prefix_len up to 2^31 - 128.  head_dim 64 or 128.
+ * dtype (q, k, v, out): bf16 or f16; scores, softmax and sums are float32, the
+ * weights are rounded to dtype for the second product.  q and out have row and
+ * head strides in elements (multiples of 2 for q, its base 4-byte aligned); out
  * may be q with equal strides.
  * A page number outside the pool, a length beyond the table's width or below 0, a
  * row_seq not below num_tables: nothing outside the pool or the table is read,

@@ -78,6 +78,8 @@ static tt_status check_prefix(const tt_shared_prefix_args* args) {
         return set_error(TT_ERR_INVALID_ARGUMENT, "shared_prefix_attention: sizes must be non-negative, num_pages positive.");
     if ((long long)a.table_width * a.page_size > INT_MAX)
         return set_error(TT_ERR_UNSUPPORTED, "shared_prefix_attention: table_width * page_size must not exceed 2^31 - 1.");
+    if (a.prefix_len > INT_MAX - kPsTile + 1)  // it is rounded up to whole key tiles
+        return set_error(TT_ERR_UNSUPPORTED, "shared_prefix_attention: prefix_len must not exceed 2^31 - 128.");
     if (!a.row_seq && a.num_tables < a.num_rows)
         return set_error(TT_ERR_INVALID_ARGUMENT, "shared_prefix_attention: without row_seq the tables need a row for each row.");
     if ((long long)a.num_rows * a.num_q_heads > (1 << 26))
