@@ -17,3 +17,19 @@ def test_a_prefix_that_does_not_round_up_is_refused(L, prefix, rows):  # noqa: F
 def test_the_longest_prefix_passes_that_check(L):  # noqa: F811
     # refused for its workspace only, after the plan
     assert status(L, "a", prefix_len=TOP - 127, page_size=32768, workspace=0) == 1 and b"workspace" in L.tt_last_error()
+
+
+@pytest.mark.parametrize("number", [1e39, -1e39, float("nan"), float("inf"), 10 ** 400, -10 ** 400])
+def test_numbers_that_no_float_holds_raise_value_errors(monkeypatch, number):
+    import torch
+    from tritiercache_b200 import _C, paged
+    # no tensor here is on a GPU: what is tested is the packing of the numbers, before any call of the library
+    monkeypatch.setattr(paged, "_device", lambda t, name: -1)
+    monkeypatch.setattr(paged, "_run", lambda *a: pytest.fail("the call went through"))
+    z = lambda *s: torch.zeros(s, dtype=torch.bfloat16)  # noqa: E731
+    i = lambda *s: torch.zeros(s, dtype=torch.int32)  # noqa: E731
+    with pytest.raises(ValueError):
+        _C.shared_prefix_attention(z(1, 2, 64), z(1, 16, 1, 64), z(1, 16, 1, 64), None, 0, i(1, 1), i(1), z(1, 2, 64), scale=number)
+    if isinstance(number, int):
+        with pytest.raises(ValueError):
+            _C.qk_norm_rope(z(1, 2, 64), z(1, 1, 64), z(1, 1, 64), None, None, z(1, 2, 64), z(1, 1, 64), z(1, 1, 64), eps=number)

@@ -75,14 +75,15 @@ def _run(fn, packed: bytes, index: int, what: str) -> None:
 
 
 def _tensors_only(fn):
-    """What is not a tensor has none of a tensor's attributes; what is no 32-bit whole number does not pack."""
+    """What is not a tensor has none of a tensor's attributes; what is no 32-bit whole number does not pack, nor does a
+    whole number that no float holds."""
     @functools.wraps(fn)
     def call(*args, **kw):
         try:
             return fn(*args, **kw)
         except AttributeError as e:
             raise ValueError(f"{fn.__name__} takes tensors: {e}") from None
-        except struct.error as e:
+        except (struct.error, OverflowError) as e:
             raise ValueError(f"{fn.__name__}: a number does not fit its type: {e}") from None
     return call
 
