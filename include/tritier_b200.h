@@ -498,6 +498,7 @@ tt_status tt_qk_norm_rope(const tt_qk_norm_rope_args* args, void* stream);
  * page * page_stride + token * token_stride + head * head_stride + channel, all
  * strides multiples of 8 elements, bases 16-byte aligned.  page_size: a power of
  * two from 16 to 32768.  prefix_len up to 2^31 - 128.  head_dim 64 or 128.
+ * scale and scale * log2(e) finite in float32.
  * dtype (q, k, v, out): bf16 or f16; scores, softmax and sums are float32, the
  * weights are rounded to dtype for the second product.  q and out have row and
  * head strides in elements (multiples of 2 for q, its base 4-byte aligned); out

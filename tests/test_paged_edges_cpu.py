@@ -19,7 +19,7 @@ def test_the_longest_prefix_passes_that_check(L):  # noqa: F811
     assert status(L, "a", prefix_len=TOP - 127, page_size=32768, workspace=0) == 1 and b"workspace" in L.tt_last_error()
 
 
-@pytest.mark.parametrize("number", [1e39, -1e39, float("nan"), float("inf"), 10 ** 400, -10 ** 400])
+@pytest.mark.parametrize("number", [1e39, -1e39, float("nan"), float("inf"), 10 ** 400, -10 ** 400], ids=lambda x: f"{x:.0e}" if isinstance(x, float) else "huge")
 def test_numbers_that_no_float_holds_raise_value_errors(monkeypatch, number):
     import torch
     from tritiercache_b200 import _C, paged
@@ -33,3 +33,10 @@ def test_numbers_that_no_float_holds_raise_value_errors(monkeypatch, number):
     if isinstance(number, int):
         with pytest.raises(ValueError):
             _C.qk_norm_rope(z(1, 2, 64), z(1, 1, 64), z(1, 1, 64), None, None, z(1, 2, 64), z(1, 1, 64), z(1, 1, 64), eps=number)
+
+
+@pytest.mark.parametrize("scale", [2.4e38, 3.4e38, -3e38])
+def test_a_scale_whose_base_two_form_is_infinite_is_refused(L, scale):  # noqa: F811
+    # scores are kept in powers of two: scale * log2(e); infinity times a score of zero would be NaN
+    assert status(L, "a", scale=scale) == 1 and b"scale" in L.tt_last_error()
+    assert status(L, "a", scale=scale / 2, workspace=0) == 1 and b"workspace" in L.tt_last_error()

@@ -85,8 +85,9 @@ static tt_status check_prefix(const tt_shared_prefix_args* args) {
     if ((long long)a.num_rows * a.num_q_heads > (1 << 26))
         return set_error(TT_ERR_UNSUPPORTED, "shared_prefix_attention: more than 2^26 query heads in one call.");
     if (a.num_q_heads > 65535) return set_error(TT_ERR_UNSUPPORTED, "shared_prefix_attention: more than 65535 query heads.");
-    if (!(a.scale > -INFINITY && a.scale < INFINITY))
-        return set_error(TT_ERR_INVALID_ARGUMENT, "shared_prefix_attention: scale must be finite.");
+    // scores are kept in log2 units
+    if (!(a.scale * kLog2e > -INFINITY && a.scale * kLog2e < INFINITY))
+        return set_error(TT_ERR_INVALID_ARGUMENT, "shared_prefix_attention: scale and scale * log2(e) must be finite.");
     if ((a.k_page_stride | a.k_token_stride | a.k_head_stride | a.v_page_stride | a.v_token_stride | a.v_head_stride) & 7)
         return set_error(TT_ERR_UNSUPPORTED, "shared_prefix_attention: strides of k and v must be multiples of 8 elements.");
     if ((a.q_row_stride | a.q_head_stride) & 1)

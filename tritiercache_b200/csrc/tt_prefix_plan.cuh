@@ -10,6 +10,7 @@ namespace tt {
 constexpr int kRowWarps = 4;     // warps of a CTA of the rows' pass
 constexpr int kGroup = 16;       // tokens per warp step
 constexpr int kPsTile = 128;     // prefix pass: keys per tile, rows per accumulator
+constexpr float kLog2e = 1.4426950408889634f;
 
 struct PrefixParams {
     tt_shared_prefix_args a;
@@ -47,7 +48,7 @@ inline size_t own_slots(const PrefixParams& p) { return p.join ? (size_t)p.split
 inline PrefixParams plan_prefix(const tt_shared_prefix_args& a) {
     PrefixParams p = {};
     p.a = a;
-    p.scale_log2 = a.scale * 1.4426950408889634f;
+    p.scale_log2 = a.scale * kLog2e;
     p.group = a.num_q_heads / a.num_kv_heads;
     while ((1 << p.page_shift) < a.page_size) ++p.page_shift;
     p.head_tiles = p.group <= 8 ? 1 : (p.group + 15) / 16;
