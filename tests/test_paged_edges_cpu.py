@@ -1,7 +1,9 @@
 """Refusals of the paged operators at the edges of their arguments' ranges (no GPU needed)."""
+import ctypes as C
+
 import pytest
 
-from test_paged_cpu import L, UNSUPPORTED, status  # noqa: F401
+from test_paged_cpu import L, UNSUPPORTED, pack, status  # noqa: F401
 
 TOP = 2 ** 31 - 1
 
@@ -39,4 +41,5 @@ def test_numbers_that_no_float_holds_raise_value_errors(monkeypatch, number):
 def test_a_scale_whose_base_two_form_is_infinite_is_refused(L, scale):  # noqa: F811
     # scores are kept in powers of two: scale * log2(e); infinity times a score of zero would be NaN
     assert status(L, "a", scale=scale) == 1 and b"scale" in L.tt_last_error()
-    assert status(L, "a", scale=scale / 2, workspace=0) == 1 and b"workspace" in L.tt_last_error()
+    n = C.c_size_t()
+    assert L.tt_shared_prefix_attention_workspace(pack("a", scale=scale / 2), C.byref(n)) == 0
