@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 import torch
 
-from test_gpu_paged import C_, same, tables_gpu, tables_ref  # noqa: F401
+from test_gpu_paged import BF, C_, attend, attn_close, make_attn, same, tables_gpu, tables_ref  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -27,3 +27,17 @@ def test_page_tables_lengths_at_the_top_of_their_type(C_, B, P):  # noqa: F811
     assert want["deferred"][0] == 3
     same(tables_gpu(C_, ctx, new, tables, free, count, P, rows, 0), want)
     same(tables_gpu(C_, ctx, new, tables, free, count, P, rows, 0, in_place=True), want)
+
+
+def test_attention_takes_any_stride_of_a_single_row_or_head(C_):  # noqa: F811
+    s = make_attn(60, 1, 8, 2, 128, 300, [20], 16, BF)
+    want = attend(C_, s)
+    attn_close(want, s, 128 ** -0.5)
+    one = s["q"].as_strided(s["q"].shape, (1025, 128, 1))
+    assert torch.equal(attend(C_, {**s, "q": one}, out=torch.empty_like(s["q"])), want)
+    for prefix in (300, 40000):  # read by the rows, and by a pass of its own
+        s = make_attn(61, 5, 1, 1, 64, prefix, [20] * 5, 16, BF)
+        want = attend(C_, s)
+        attn_close(want, s, 64 ** -0.5)
+        one = s["q"].as_strided(s["q"].shape, (64, 67, 1))
+        assert torch.equal(attend(C_, {**s, "q": one}, out=torch.empty_like(s["q"])), want)

@@ -215,9 +215,10 @@ def shared_prefix_attention(q, k_pages, v_pages, prefix_table, prefix_len, table
     """Decode attention of a batch over a prefix that all rows share, read once
     for all of them, and over each row's own pages.
 
-    ``q``, ``out`` [rows, q_heads, head_dim]; ``k_pages``/``v_pages`` [pages,
-    page_size, kv_heads, head_dim] (any strides that keep channels contiguous and
-    16-byte steps; bfloat16 or float16 throughout).  Row r attends tokens
+    ``q``, ``out`` [rows, q_heads, head_dim], channels contiguous, strides and
+    start of q multiples of 2 elements; ``k_pages``/``v_pages`` [pages, page_size,
+    kv_heads, head_dim], channels contiguous, other strides and start in 16-byte
+    steps, page_size a power of two from 16; bfloat16 or float16 throughout.  Row r attends tokens
     [0, prefix_len) of the pages in ``prefix_table`` and tokens [0, row_lens[r])
     of the pages in row ``row_seq[r]`` (None: r) of ``tables``.  ``scale``
     defaults to head_dim ** -0.5.  Rows with row_seq < 0 are padding and stay as
@@ -237,7 +238,9 @@ def shared_prefix_attention(q, k_pages, v_pages, prefix_table, prefix_len, table
     qs, os = _rows(q, "q", index, dt, shape), _rows(out, "out", index, dt, shape)
     _apart(out, os, "out")
     ks, vs = _rows(k_pages, "k_pages", index, dt, pool), _rows(v_pages, "v_pages", index, dt, pool)
-    if 1 in pool:  # the stride of a dimension of one entry says nothing
+    if R == 1 or nq == 1:  # the stride of a dimension of one entry says nothing
+        qs = tuple(d if n > 1 else hd for n, d in zip(shape, qs))
+    if 1 in pool:
         ks, vs = (tuple(d if n > 1 else hd for n, d in zip(pool, st)) for st in (ks, vs))
     ppt, have = 0, 0
     if prefix_table is not None:
