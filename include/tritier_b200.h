@@ -527,6 +527,12 @@ typedef struct {
 } tt_shared_prefix_args;
 tt_status tt_shared_prefix_attention_workspace(const tt_shared_prefix_args* args, size_t* bytes);
 tt_status tt_shared_prefix_attention(const tt_shared_prefix_args* args, void* stream);
+/* Every wait inside these kernels is bounded, by about two seconds.  When one
+ * runs out, the rows that needed it come out NaN and tt_device_error reports
+ * TT_ERR_TIMEOUT.  This sets the bound, in GPU clocks, for this process's later
+ * calls (graphs keep the one they were captured with): for tests of that path.
+ * Negative, or above the two seconds: two seconds again. */
+tt_status tt_shared_prefix_wait_limit(int64_t clocks);
 
 #if defined(__GNUC__)
 #pragma GCC visibility pop

@@ -67,7 +67,7 @@ EXPORTS = [
     "tt_sharded_xch_open", "tt_sharded_xch_destroy", "tt_engine_step_sharded_begin_xch",
     "tt_engine_step_sharded_merge_xch",
     "tt_page_tables_workspace", "tt_page_tables", "tt_qk_norm_rope", "tt_shared_prefix_attention_workspace",
-    "tt_shared_prefix_attention",
+    "tt_shared_prefix_attention", "tt_shared_prefix_wait_limit",
     "tt_engine_ingest", "tt_engine_full_count", "tt_engine_reconstruct", "tt_engine_accumulate_scores",
 ]
 
@@ -127,6 +127,7 @@ def _declare(L):
     L.tt_qk_norm_rope.argtypes = [vp, vp]
     L.tt_shared_prefix_attention_workspace.argtypes = [vp, C.POINTER(C.c_size_t)]
     L.tt_shared_prefix_attention.argtypes = [vp, vp]
+    L.tt_shared_prefix_wait_limit.argtypes = [C.c_int64]
     for name in EXPORTS:
         if name not in ("tt_last_error", "tt_version", "tt_page_tables_workspace"):
             getattr(L, name).restype = C.c_int

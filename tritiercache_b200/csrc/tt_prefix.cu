@@ -103,6 +103,8 @@ static tt_status check_prefix(const tt_shared_prefix_args* args) {
     return TT_OK;
 }
 
+static std::atomic<long long> g_wait_limit{kPatience};
+
 // The pool in boxes of 64 channels and `tokens` tokens of one head.
 using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                               const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
@@ -172,11 +174,17 @@ tt_status tt_shared_prefix_attention_workspace(const tt_shared_prefix_args* args
     return TT_OK;
 }
 
+tt_status tt_shared_prefix_wait_limit(int64_t clocks) {
+    g_wait_limit.store(clocks < 0 || clocks > kPatience ? kPatience : (long long)clocks, std::memory_order_relaxed);
+    return TT_OK;
+}
+
 tt_status tt_shared_prefix_attention(const tt_shared_prefix_args* args, void* stream) {
     const tt_status s = check_prefix(args);
     if (s != TT_OK) return s;
     if (args->num_rows == 0) return TT_OK;
     PrefixParams p = plan_prefix(*args);
+    p.patience = g_wait_limit.load(std::memory_order_relaxed);
     const tt_shared_prefix_args& a = p.a;
     const bool bf = a.dtype == TT_DTYPE_BF16;
     const cudaStream_t st = (cudaStream_t)stream;

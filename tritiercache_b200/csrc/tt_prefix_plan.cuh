@@ -15,6 +15,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 struct PrefixParams {
     tt_shared_prefix_args a;
     float scale_log2;            // scale * log2(e)
+    long long patience;          // clocks that a wait may take before the CTA gives up
     int page_shift;
     int group;                   // query heads per kv head
     int head_tiles;              // tiles of 8*NB query heads per kv head

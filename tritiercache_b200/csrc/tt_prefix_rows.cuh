@@ -38,6 +38,12 @@ constexpr long long kPatience = 4000000000LL;  // clocks that a wait may take (a
 
 __device__ int g_prefix_error = 0;  // a wait that ran out (TT_ERR_TIMEOUT); reported by tt_device_error
 
+struct WaitState {           // in shared memory, of those that give up together: a warp here, a CTA in the prefix pass
+    long long limit;         // clocks that a wait may take (in constant memory it cost 0.3 us of every call)
+    int abort;
+    int pad;
+};
+
 template <typename T> __device__ __forceinline__ void mma16816(float* c, const uint32_t* a, uint32_t b0, uint32_t b1);
 template <>
 __device__ __forceinline__ void mma16816<__nv_bfloat16>(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
@@ -99,24 +105,33 @@ __device__ __forceinline__ bool bar_try(uint32_t b, uint32_t parity) {
                  : "=r"(ok) : "r"(b), "r"(parity) : "memory");
     return ok != 0;
 }
-// Bounded: false when it took too long here (recorded) or elsewhere in the CTA.
-__device__ __noinline__ bool bar_wait_slow(uint32_t b, uint32_t parity, volatile int* abort) {
-    const long long t0 = clock64();
-    while (clock64() - t0 < kPatience) {
+// Bounded: false when it took too long here (recorded) or elsewhere.
+__device__ __noinline__ bool bar_wait_slow(uint32_t b, uint32_t parity, volatile WaitState* w) {
+    const long long t0 = clock64(), limit = w->limit;
+    while (clock64() - t0 < limit) {
         if (bar_try(b, parity)) return true;
-        if (abort && *abort) return false;
+        if (w->abort) return false;
     }
-    if (abort) *abort = 1;
+    w->abort = 1;
     atomicCAS(&g_prefix_error, 0, (int)TT_ERR_TIMEOUT);
     return false;
 }
-__device__ __forceinline__ bool bar_wait(uint32_t b, uint32_t parity, volatile int* abort) {
-    return bar_try(b, parity) || bar_wait_slow(b, parity, abort);
+__device__ __forceinline__ bool bar_wait(uint32_t b, uint32_t parity, volatile WaitState* w) {
+    return bar_try(b, parity) || bar_wait_slow(b, parity, w);
+}
+// The wait for copies or products in flight, before their memory is given back: whatever the limit, kPatience.
+__device__ __noinline__ void bar_drain(uint32_t b, uint32_t parity) {
+    const long long t0 = clock64();
+    while (!bar_try(b, parity))
+        if (clock64() - t0 > kPatience) {
+            atomicCAS(&g_prefix_error, 0, (int)TT_ERR_TIMEOUT);
+            return;
+        }
 }
 
 // The same by a whole warp, with one answer.
-__device__ __forceinline__ bool bar_wait_warp(uint32_t b, uint32_t parity, volatile int* abort) {
-    return __all_sync(~0u, bar_wait(b, parity, abort));
+__device__ __forceinline__ bool bar_wait_warp(uint32_t b, uint32_t parity, volatile WaitState* w) {
+    return __all_sync(~0u, bar_wait(b, parity, w));
 }
 
 // A box of the pool: channel, head, token in page, page.  Outside the pool it is zeros.
@@ -225,7 +240,9 @@ template <int HD, int NB, int ST> constexpr int row_warp_bytes() {
     static_assert(ST * 2 * kGroup * HD * 2 >= row_out_bytes<HD, NB>(), "the partials take the stages' place");
     return ST * 2 * kGroup * HD * 2;
 }
-template <int HD, int NB, int ST> constexpr int row_smem() { return kRowWarps * (row_warp_bytes<HD, NB, ST>() + 2 * ST * 8); }
+template <int HD, int NB, int ST> constexpr int row_smem() {
+    return kRowWarps * (row_warp_bytes<HD, NB, ST>() + 2 * ST * 8 + (int)sizeof(WaitState));
+}
 
 template <typename T, int HD, int NB, int ST>
 __global__ void __launch_bounds__(kRowWarps * 32, 4)
@@ -264,7 +281,10 @@ k_prefix_rows(const PrefixParams p, const __grid_constant__ CUtensorMap kmap, co
 
     const uint32_t base = smem_addr(sm) + warp * kWarp;
     const uint32_t bars = smem_addr(sm) + kRowWarps * kWarp + warp * 2 * ST * 8;  // K of each stage, V of each stage
+    volatile WaitState* wait = reinterpret_cast<WaitState*>(sm + kRowWarps * (kWarp + 2 * ST * 8)) + warp;
     if (lane == 0) {
+        wait->limit = p.patience;
+        wait->abort = 0;
         for (int i = 0; i < 2 * ST; ++i) bar_init(bars + 8 * i, 1);
         asm volatile("fence.mbarrier_init.release.cluster;\nfence.proxy.async.shared::cta;" ::: "memory");
     }
@@ -332,7 +352,7 @@ k_prefix_rows(const PrefixParams p, const __grid_constant__ CUtensorMap kmap, co
     int g = g0;
     for (; g < groups; g += step) {
         const uint32_t kd = base + stage * 2 * kTile, vd = kd + kTile;
-        if (!bar_wait_warp(bars + 8 * stage, phase, nullptr)) {
+        if (!bar_wait_warp(bars + 8 * stage, phase, wait)) {
             lost = true;
             break;
         }
@@ -393,7 +413,7 @@ k_prefix_rows(const PrefixParams p, const __grid_constant__ CUtensorMap kmap, co
             pb[nb][0] = movm_t(pack2<T>(p0, p1));
             pb[nb][1] = movm_t(pack2<T>(p2, p3));
         }
-        if (!bar_wait_warp(bars + 8 * (ST + stage), phase, nullptr)) {
+        if (!bar_wait_warp(bars + 8 * (ST + stage), phase, wait)) {
             lost = true;
             k_next = g_issue < groups;
             break;
@@ -433,9 +453,9 @@ k_prefix_rows(const PrefixParams p, const __grid_constant__ CUtensorMap kmap, co
         bad = true;
         for (int i = 0; i < 2 * ST; ++i) {
             const int st = (stage + i / 2) % ST;
-            if (g + (i / 2) * step < groups) bar_wait_slow(bars + 8 * ((i & 1) * ST + st), phase ^ (st < stage), nullptr);
+            if (g + (i / 2) * step < groups) bar_drain(bars + 8 * ((i & 1) * ST + st), phase ^ (st < stage));
         }
-        if (k_next) bar_wait_slow(bars + 8 * stage, phase ^ 1, nullptr);
+        if (k_next) bar_drain(bars + 8 * stage, phase ^ 1);
         __syncwarp();
     }
 

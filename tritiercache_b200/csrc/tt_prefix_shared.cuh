@@ -47,8 +47,9 @@ template <int HD, bool PAIR> struct PsShape {
 
 struct PsBars {  // in shared memory
     uint64_t full[8], empty[8], q_full, s_full[2], p_ready[4], v_cut, v_fixed, drain;
-    uint32_t tmem;
-    int abort, bad;
+    WaitState wait;
+    uint32_t tmem, loads;
+    int bad;
 };
 
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -136,7 +137,7 @@ k_prefix_shared(const PrefixParams p, const __grid_constant__ CUtensorMap kmap, 
     const uint32_t q_s = smem_addr(sm), ring = q_s + S::kQ;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const tt_shared_prefix_args& a = p.a;
-    volatile int* abort = &bars->abort;
+    volatile WaitState* wait = &bars->wait;
     const uint32_t full = smem_addr(bars->full), empty = smem_addr(bars->empty), q_full = smem_addr(&bars->q_full),
                    s_full = smem_addr(bars->s_full), p_ready = smem_addr(bars->p_ready), v_cut = smem_addr(&bars->v_cut),
                    v_fixed = smem_addr(&bars->v_fixed), drain = smem_addr(&bars->drain);
@@ -155,7 +156,8 @@ k_prefix_shared(const PrefixParams p, const __grid_constant__ CUtensorMap kmap, 
         bar_init(v_cut, 1);
         bar_init(v_fixed, 32);
         bar_init(drain, 1);
-        bars->abort = 0;
+        bars->wait.limit = p.patience;
+        bars->wait.abort = 0;
         bars->bad = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -189,7 +191,7 @@ k_prefix_shared(const PrefixParams p, const __grid_constant__ CUtensorMap kmap, 
                     }
                 }
                 const uint32_t slot = it % S::kSlots, phase = (it / S::kSlots) & 1;
-                if (!bar_wait_warp(empty + 8 * slot, phase ^ 1, abort)) return false;
+                if (!bar_wait_warp(empty + 8 * slot, phase ^ 1, wait)) return false;
                 if (lane == 0) bar_expect(full + 8 * slot, use * box * HD * 2);
                 __syncwarp();
                 if (lane < use) {
@@ -209,16 +211,14 @@ k_prefix_shared(const PrefixParams p, const __grid_constant__ CUtensorMap kmap, 
             }
             return true;
         });
-        if (*abort)  // no copy may be in flight when the CTA ends
-            for (uint32_t i = it > S::kSlots ? it - S::kSlots : 0; i < it; ++i)
-                bar_wait_slow(full + 8 * (i % S::kSlots), (i / S::kSlots) & 1, nullptr);
+        bars->loads = it;
     } else if (warp == 1) {
         // ---- the matrix instructions, from one thread
         if (elect_one()) {
             constexpr uint32_t id_qk = ps_idesc<T>(kPsTile, false), id_pv = ps_idesc<T>(HD, true);
             uint32_t it = 0, q_phase = 0, fix_phase = 0, p_phase[2] = {0, 0};
             const auto slot_of = [&](uint32_t i) { return ring + (i % S::kSlots) * S::kSlot; };
-            const auto slot_full = [&](uint32_t i) { return bar_wait(full + 8 * (i % S::kSlots), (i / S::kSlots) & 1, abort); };
+            const auto slot_full = [&](uint32_t i) { return bar_wait(full + 8 * (i % S::kSlots), (i / S::kSlots) & 1, wait); };
             const auto qk = [&](int t, uint32_t i) {
                 const uint64_t q = smem_desc(q_s + (PAIR ? t * S::kSlot : 0), 16, 1024), k = smem_desc(slot_of(i), 16, 1024);
 #pragma unroll
@@ -236,7 +236,7 @@ k_prefix_shared(const PrefixParams p, const __grid_constant__ CUtensorMap kmap, 
                 }
             };
             ps_spans(p, [&](int kvh, int tile, long long slot_at, int k0, int n) {
-                if (!bar_wait(q_full, q_phase, abort)) return false;
+                if (!bar_wait(q_full, q_phase, wait)) return false;
                 q_phase ^= 1;
                 tc_fence_after();
                 const bool cut = k0 + n == p.kv_tiles && a.prefix_len % kPsTile;
@@ -257,14 +257,14 @@ k_prefix_shared(const PrefixParams p, const __grid_constant__ CUtensorMap kmap, 
                     if (!slot_full(vi)) return false;
                     if (cut && j == n - 1) {
                         bar_arrive(v_cut);
-                        if (!bar_wait(v_fixed, fix_phase, abort)) return false;
+                        if (!bar_wait(v_fixed, fix_phase, wait)) return false;
                         fix_phase ^= 1;
                     }
                     for (int t = PAIR ? 0 : j & 1; t < (PAIR ? 2 : (j & 1) + 1); ++t) {
-                        if (!bar_wait(p_ready + 16 * t, p_phase[t], abort)) return false;
+                        if (!bar_wait(p_ready + 16 * t, p_phase[t], wait)) return false;
                         tc_fence_after();
                         pv(t, vi, 0, PAIR ? j > 0 : j > 1);
-                        if (!bar_wait(p_ready + 16 * t + 8, p_phase[t], abort)) return false;
+                        if (!bar_wait(p_ready + 16 * t + 8, p_phase[t], wait)) return false;
                         p_phase[t] ^= 1;
                         tc_fence_after();
                         pv(t, vi, 1, true);
@@ -282,7 +282,7 @@ k_prefix_shared(const PrefixParams p, const __grid_constant__ CUtensorMap kmap, 
             });
             // every product and every arrival above has happened before the CTA gives its memory back
             tc_commit(drain);
-            bar_wait_slow(drain, 0, nullptr);
+            bar_drain(drain, 0);
         }
         __syncwarp();
     } else if (warp == 2) {
@@ -292,7 +292,7 @@ k_prefix_shared(const PrefixParams p, const __grid_constant__ CUtensorMap kmap, 
             ps_spans(p, [&](int kvh, int tile, long long slot_at, int k0, int n) {
                 loads += 2 * n;
                 if (k0 + n != p.kv_tiles) return true;
-                if (!bar_wait_warp(v_cut, phase, abort)) return false;
+                if (!bar_wait_warp(v_cut, phase, wait)) return false;
                 phase ^= 1;
                 const int from = a.prefix_len % kPsTile * 8;
                 unsigned char* v = sm + S::kQ + (loads - 1) % S::kSlots * S::kSlot;  // the span's last load
@@ -339,11 +339,11 @@ k_prefix_shared(const PrefixParams p, const __grid_constant__ CUtensorMap kmap, 
             // phase that itself waits for the warp.  With no tile in this span it waits for the others' arrivals, lest
             // it arrive twice in one phase.
             bar_arrive(q_full);
-            if (!PAIR && mine == 0 && !bar_wait_warp(q_full, q_phase, abort)) return false;
+            if (!PAIR && mine == 0 && !bar_wait_warp(q_full, q_phase, wait)) return false;
             q_phase ^= 1;
             float m = -INFINITY, l = 0.f;
             for (int i = 0; i < mine; ++i) {
-                if (!bar_wait_warp(s_full + 8 * t, phase, abort)) return false;
+                if (!bar_wait_warp(s_full + 8 * t, phase, wait)) return false;
                 phase ^= 1;
                 tc_fence_after();
                 // The upper half of S goes through the registers for its maximum only; the lower half stays in them,
@@ -424,7 +424,7 @@ k_prefix_shared(const PrefixParams p, const __grid_constant__ CUtensorMap kmap, 
             // the span's partial
             const long long slot = 2 * slot_at + t;
             if (mine > 0) {
-                if (!bar_wait_warp(s_full + 8 * t, phase, abort)) return false;
+                if (!bar_wait_warp(s_full + 8 * t, phase, wait)) return false;
                 phase ^= 1;
                 tc_fence_after();
                 if (warp_on) {
@@ -446,7 +446,7 @@ k_prefix_shared(const PrefixParams p, const __grid_constant__ CUtensorMap kmap, 
             if (mrow < rows_all) p.part_ml[slot * kPsTile + row] = make_float2(m, *(volatile int*)&bars->bad ? NAN : l);
             return true;
         });
-        if (*abort) {
+        if (wait->abort) {
             // a wait ran out: nothing that this CTA was to leave may be taken for a result
             ps_spans(p, [&](int kvh, int tile, long long slot_at, int k0, int n) {
                 p.part_ml[(2 * slot_at + t) * kPsTile + row] = make_float2(-INFINITY, NAN);
@@ -455,6 +455,12 @@ k_prefix_shared(const PrefixParams p, const __grid_constant__ CUtensorMap kmap, 
         }
     }
     __syncthreads();
+    if (warp == 0 && wait->abort) {
+        // whichever warp gave up, no copy may be in flight when the CTA ends: the last load of each slot
+        const uint32_t it = bars->loads;
+        for (uint32_t i = it > S::kSlots ? it - S::kSlots : 0; i < it; ++i)
+            bar_drain(full + 8 * (i % S::kSlots), (i / S::kSlots) & 1);
+    }
     if (warp == 1) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
