@@ -62,3 +62,24 @@ def test_waits_that_run_out(C_, limit, R, nq, nkv, hd, prefix, own, P, dt):  # n
         # the next call is sound
         set_limit(-1)
         assert torch.equal(attend(C_, s), good) and error() == 0
+
+
+@pytest.mark.parametrize("R,nq,nkv,hd,prefix,own,P,dt", [(8, 96, 96, 128, 2000, 300, 16, BF), (256, 32, 8, 128, 16400, 300, 32, BF),
+                                                          (256, 16, 4, 64, 16400, 700, 32, F16)])
+def test_giving_up_takes_no_time(C_, limit, R, nq, nkv, hd, prefix, own, P, dt):  # noqa: F811
+    """What is in flight when a warp gives up arrives within microseconds; nothing waits for what has been before."""
+    set_limit, error = limit
+    s = make_attn(71, R, nq, nkv, hd, prefix, np.full(R, own), P, dt)
+    attend(C_, s)
+    slowest = 0.0
+    a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+    for clocks in (0, 1, 100, 300, 1000):
+        set_limit(clocks)
+        for _ in range(8):
+            a.record()
+            attend(C_, s)
+            b.record()
+            torch.cuda.synchronize()
+            slowest = max(slowest, a.elapsed_time(b))
+        assert error() == TIMEOUT
+    assert slowest < 500, slowest  # milliseconds; a wait in vain takes 2000

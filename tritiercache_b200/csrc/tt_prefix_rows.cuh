@@ -348,7 +348,7 @@ k_prefix_rows(const PrefixParams p, const __grid_constant__ CUtensorMap kmap, co
 
     int stage = 0;
     uint32_t phase = 0;
-    bool lost = false, k_next = false;  // a wait ran out; the stage's next K has been asked for
+    bool lost = false, at_v = false;  // a wait ran out; it was for V, with K used and the stage's next one asked for
     int g = g0;
     for (; g < groups; g += step) {
         const uint32_t kd = base + stage * 2 * kTile, vd = kd + kTile;
@@ -415,7 +415,7 @@ k_prefix_rows(const PrefixParams p, const __grid_constant__ CUtensorMap kmap, co
         }
         if (!bar_wait_warp(bars + 8 * (ST + stage), phase, wait)) {
             lost = true;
-            k_next = g_issue < groups;
+            at_v = true;
             break;
         }
         if (n < kGroup) {
@@ -453,9 +453,10 @@ k_prefix_rows(const PrefixParams p, const __grid_constant__ CUtensorMap kmap, co
         bad = true;
         for (int i = 0; i < 2 * ST; ++i) {
             const int st = (stage + i / 2) % ST;
-            if (g + (i / 2) * step < groups) bar_drain(bars + 8 * ((i & 1) * ST + st), phase ^ (st < stage));
+            const bool next = at_v && i == 0;  // a phase that is long past would be waited for in vain
+            if (next ? g_issue < groups : g + (i / 2) * step < groups)
+                bar_drain(bars + 8 * ((i & 1) * ST + st), phase ^ (next || st < stage));
         }
-        if (k_next) bar_drain(bars + 8 * stage, phase ^ 1);
         __syncwarp();
     }
 
