@@ -43,3 +43,16 @@ def test_a_scale_whose_base_two_form_is_infinite_is_refused(L, scale):  # noqa: 
     assert status(L, "a", scale=scale) == 1 and b"scale" in L.tt_last_error()
     n = C.c_size_t()
     assert L.tt_shared_prefix_attention_workspace(pack("a", scale=scale / 2), C.byref(n)) == 0
+
+
+@pytest.mark.parametrize("kw", [dict(dtype="float32"), dict(dtype="float64"), dict(head_dim=96), dict(head_dim=256),
+                                dict(page_size=48), dict(page_size=8), dict(page_size=65536), dict(max_pages=1 << 27, page_size=16),
+                                dict(num_pages=0), dict(max_rows=0)])
+def test_a_batch_that_could_not_attend_is_refused_when_it_is_made(kw):
+    import torch
+    from tritiercache_b200 import SharedPrefixBatch
+    ok = dict(num_pages=8, page_size=16, num_kv_heads=1, head_dim=64, max_requests=2, max_pages=4, max_rows=2, dtype="bfloat16")
+    args = {**ok, **kw}
+    args["dtype"] = getattr(torch, args["dtype"])
+    with pytest.raises(ValueError):
+        SharedPrefixBatch(device="cpu", **args)

@@ -287,7 +287,8 @@ class SharedPrefixBatch:
         batch.attend(q_out, out)                    # prompt once for all rows, then each row's own pages
 
     The buffers belong to the object and keep their addresses, so a step can be
-    captured into a CUDA graph.  No reference counterpart.  ``max_rows`` is the
+    captured into a CUDA graph.  bfloat16 or float16, head_dim 64 or 128, pages of
+    a power of two from 16 tokens.  No reference counterpart.  ``max_rows`` is the
     number of new tokens a step can hold; rows behind the step's are padding.
     After ``begin``: ``lens`` [requests] tokens held, ``row_seq`` [rows] the
     request of each row (-1: padding), ``deferred`` [1] the requests that found
@@ -298,6 +299,15 @@ class SharedPrefixBatch:
                  dtype=torch.bfloat16, device=None):
         if min(num_pages, page_size, num_kv_heads, head_dim, max_requests, max_pages, max_rows) <= 0:
             raise ValueError("sizes must be positive.")
+        # what attend() takes, said before the buffers are made
+        if dtype is not _BF16 and dtype is not _F16:
+            raise ValueError(f"dtype must be bfloat16 or float16, got {dtype}.")
+        if head_dim not in (64, 128):
+            raise ValueError(f"head_dim must be 64 or 128, got {head_dim}.")
+        if not 16 <= page_size <= 32768 or page_size & (page_size - 1):
+            raise ValueError(f"page_size must be a power of two from 16 to 32768, got {page_size}.")
+        if max_pages * page_size > 2 ** 31 - 1:
+            raise ValueError("max_pages * page_size must not exceed 2^31 - 1.")
         device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
         shape = (num_pages, page_size, num_kv_heads, head_dim)
         self.k_pages, self.v_pages = (torch.zeros(shape, dtype=dtype, device=device) for _ in range(2))
