@@ -27,7 +27,8 @@ SCORE_DECAY = 0.999
 K_GROUP_SIZE = 16
 PBS_METADATA_DTYPE = "fp16"
 # Decode steps: norm, rotation and the float32 rows of q, k and v in one kernel (qk_norm_rope) with one rounding
-# instead of the module's own steps in its dtype.  Set by apply_patch(fused_qk=True).
+# instead of the module's own steps in its dtype.  Set by apply_patch(fused_qk=True).  Modules whose norms have hooks or
+# a replaced forward keep their own steps.
 FUSED_QK = False
 
 
@@ -57,13 +58,27 @@ def _reference_attention_path(self, cache: TriTierCache, Q: torch.Tensor, num_q_
     return torch.matmul(w, V_full).to(Q.device), w.to(Q.device)
 
 
+_HOOKS = ("_forward_hooks", "_forward_pre_hooks", "_backward_hooks", "_backward_pre_hooks")
+_GLOBAL_HOOKS = ("_global_forward_hooks", "_global_forward_pre_hooks", "_global_backward_hooks", "_global_backward_pre_hooks")
+
+
+def _plain_norm(n, hd: int) -> bool:
+    """An RMS norm over head_dim that the kernel may stand in for: nobody watches its calls or has replaced its
+    forward."""
+    return (hasattr(n, "variance_epsilon") and n.weight.shape == (hd,) and "forward" not in vars(n) and
+            not any(getattr(n, h, None) for h in _HOOKS) and
+            not any(getattr(torch.nn.modules.module, h, None) for h in _GLOBAL_HOOKS))
+
+
 def _fused_rows(self, q, k, v, cos, sin, device):
     """The float32 rows (Q, K, V) of one decode token by qk_norm_rope, or None where the module's norms or types
     are not the kernel's."""
     hd = q.shape[-1]
     norms = [getattr(self, "q_norm", None), getattr(self, "k_norm", None)]
-    eps = {float(n.variance_epsilon) for n in norms if n is not None and hasattr(n, "variance_epsilon")}
-    if len(eps) > 1 or any(n is not None and not (hasattr(n, "variance_epsilon") and n.weight.shape == (hd,)) for n in norms):
+    if any(n is not None and not _plain_norm(n, hd) for n in norms):
+        return None
+    eps = {float(n.variance_epsilon) for n in norms if n is not None}
+    if len(eps) > 1:
         return None
     w = [None if n is None else n.weight.detach() for n in norms]
     types = {t.dtype for t in w if t is not None}
