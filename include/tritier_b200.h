@@ -500,7 +500,9 @@ tt_status tt_qk_norm_rope(const tt_qk_norm_rope_args* args, void* stream);
  * two from 16 to 32768.  prefix_len up to 2^31 - 128.  head_dim 64 or 128.
  * scale and scale * log2(e) finite in float32.
  * dtype (q, k, v, out): bf16 or f16; scores, softmax and sums are float32, the
- * weights are rounded to dtype for the second product.  q and out have row and
+ * weights are rounded to dtype for the second product, whose float32 sums drop
+ * products below 2^-25 of themselves: keys so far under the largest score add
+ * nothing to the output while they count in its denominator.  q and out have row and
  * head strides in elements (multiples of 2 for q, its base 4-byte aligned); out
  * may be q with equal strides.
  * A page number outside the pool, a length beyond the table's width or below 0, a

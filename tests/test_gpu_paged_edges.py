@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 import torch
 
-from test_gpu_paged import BF, C_, attend, attn_close, make_attn, same, tables_gpu, tables_ref  # noqa: F401
+from test_gpu_paged import BF, C_, F16, attend, attn_close, make_attn, same, tables_gpu, tables_ref  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -41,3 +41,33 @@ def test_attention_takes_any_stride_of_a_single_row_or_head(C_):  # noqa: F811
         attn_close(want, s, 64 ** -0.5)
         one = s["q"].as_strided(s["q"].shape, (64, 67, 1))
         assert torch.equal(attend(C_, {**s, "q": one}, out=torch.empty_like(s["q"])), want)
+
+
+@pytest.mark.parametrize("dt", [BF, F16])
+@pytest.mark.parametrize("where", ["prefix", "own"])
+@pytest.mark.parametrize("bits", [0, 20, 25.6, 40])
+def test_attention_over_many_keys_far_below_the_largest(C_, dt, where, bits):  # noqa: F811
+    """One key `bits` powers of two above 2^18 or 2^20 others, all values 1, so the exact output is 1.  A product below
+    2^-25 of a tensor core's accumulator may add nothing to it, while its weight counts in the denominator: that is the
+    most that may be lost."""
+    P, hd = 1024, 64
+    nkv, R, n = (160, 2, 2 ** 18) if where == "prefix" else (1, 300, 2 ** 20)
+    k = torch.zeros((2, P, nkv, hd), device="cuda", dtype=dt)
+    k[0, 0, :, 0] = 1.0  # the first key of page 0; page 1 holds zeros
+    v = torch.ones_like(k)
+    q = torch.zeros((R, nkv, hd), device="cuda", dtype=dt)
+    q[..., 0] = 1.0
+    table = torch.ones(n // P, device="cuda", dtype=torch.int32)
+    table[0] = 0
+    none = torch.zeros((R, 1), device="cuda", dtype=torch.int32)
+    lens = torch.zeros(R, device="cuda", dtype=torch.int32)
+    out = torch.zeros_like(q)
+    scale = max(bits, 2.0 ** -20) * np.log(2.0)
+    if where == "prefix":
+        C_.shared_prefix_attention(q, k, v, table, n, none, lens, out, scale=scale)
+    else:
+        C_.shared_prefix_attention(q, k, v, None, 0, table.expand(R, -1), lens + n, out, scale=scale)
+    # the last rounding; the weights' (all of one size, a power of two but for bits = 25.6, where they are lost);
+    # what is lost; float32 sums of parts of n numbers, each rounded by 2^-24 of the sum so far
+    lim = torch.finfo(dt).eps / 2 + (n * 2.0 ** -bits if bits > 25 else 0) + n / 16 * 2.0 ** -24
+    assert float((out.double() - 1).abs().max()) <= lim
