@@ -491,7 +491,7 @@ tt_status tt_qk_norm_rope(const tt_qk_norm_rope_args* args, void* stream);
  * query head h on kv head h / (num_q_heads / num_kv_heads).  Several new tokens
  * of one request are several rows with their own row_lens.  A row with
  * row_seq[r] < 0 is padding and its output stays as it was; a row with nothing
- * to attend gives zeros.  Keys and values behind a length are not used, whatever
+ * to attend, or with no score above -infinity, gives zeros.  Keys and values behind a length are not used, whatever
  * they hold.
  *
  * k and v: pools of num_pages pages, element (page, token, head, channel) at

@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 import torch
 
-from test_gpu_paged import BF, C_, F16, attend, attn_close, make_attn, same, tables_gpu, tables_ref  # noqa: F401
+from test_gpu_paged import BF, C_, F16, attend, attn_close, attn_ref, make_attn, same, tables_gpu, tables_ref  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -71,3 +71,21 @@ def test_attention_over_many_keys_far_below_the_largest(C_, dt, where, bits):  #
     # what is lost; float32 sums of parts of n numbers, each rounded by 2^-24 of the sum so far
     lim = torch.finfo(dt).eps / 2 + (n * 2.0 ** -bits if bits > 25 else 0) + n / 16 * 2.0 ** -24
     assert float((out.double() - 1).abs().max()) <= lim
+
+
+@pytest.mark.parametrize("dt", [BF, F16])
+@pytest.mark.parametrize("R,prefix", [(3, 40), (60, 1500)])  # the rows read the prefix, and a pass of its own
+def test_attention_with_scores_of_minus_infinity(C_, dt, R, prefix):  # noqa: F811
+    s = make_attn(62, R, 8, 4, 64, prefix, [40] * R, 16, dt)
+    s["q"][..., 0] = 1.0
+    s["k"][..., 0][s["k"][..., 1] > 0.5] = float("-inf")  # such keys have no weight
+    # as attn_close, with the reach of the other keys
+    got = attend(C_, s)
+    want, mag, _ = attn_ref(s, 64 ** -0.5)
+    finite = s["k"].double().where(s["k"] > float("-inf"), 0.0)
+    reach = float(s["q"].double().norm(dim=-1).max() * finite.norm(dim=-1).max()) / 8
+    u = torch.finfo(dt).eps / 2
+    lim = u * want.abs() + mag * (u + 2 * 64 * 2.0 ** -23 * reach + 2.0 ** -20) * 1.01 + (prefix + 40) * 2.0 ** -22 * (dt == F16)
+    assert bool(torch.isfinite(want).all()) and bool(((got.double() - want).abs() <= lim).all())
+    s["k"][..., 0] = float("-inf")  # nothing left: zeros, as of a row with nothing to attend
+    assert bool((attend(C_, s) == 0).all())

@@ -29,6 +29,7 @@ CROSSING = [
     (300, 48, 48, 128, 1999, 10, 16, BF, 1, "nhd"),
     (600, 16, 2, 128, 9001, 10, 32, F16, 1, "nhd"),   # 19 row tiles
     (600, 16, 2, 64, 9100, 10, 16, BF, 3, "hnd"),
+    (5000, 8, 1, 64, 300, 3, 16, BF, 1, "nhd"),       # more row tiles than CTAs
 ]
 
 

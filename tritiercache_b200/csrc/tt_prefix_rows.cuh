@@ -3,7 +3,7 @@
 //
 // `splits` CTAs per (row, kv head, tile of up to 8*NB query heads).  Their 4*splits warps take the row's
 // tokens in groups of 16 (a group never crosses a page), warp w groups w, w+4*splits, ...; each warp keeps its
-// own cp.async pipeline of K and V groups, so no warp waits for another before the end.  Per group, with
+// own pipeline of K and V groups, so no warp waits for another before the end.  Per group, with
 // mma.sync m16n8k16 and tokens along M, because a row has few query heads and 16 tokens:
 //   S^T[16 x 8] = K[16 x hd] Q^T[hd x 8]         (K by ldmatrix, Q^T in registers)
 //   P^T = 2^(S^T - m), transposed in registers (movmatrix) into the second product's B operand
@@ -18,10 +18,12 @@
 //
 // Loads are TMA boxes of 16 tokens (cp.async by the lanes instead cost the warps a third of their instructions,
 // and beside the prefix pass more: 282 against 257 us for 256 rows on 32k).  Weights are rounded to the pages'
-// type for the second product, as in the prefix pass; logits, exponentials and sums are float32.
+// type for the second product, as in the prefix pass; logits, exponentials and sums are float32 (a product below
+// 2^-25 of its sum is dropped by the tensor cores, while its weight counts in l).
 //
 // Bound: HBM (each row's K and V are read once).  Alone, 256 rows of up to 2048 tokens (1.08 GB): 170 us,
-// 6.3 TB/s.
+// 6.3 TB/s.  More than eight query heads a kv head take two fragments of everything and spill 44 bytes at 128
+// registers a thread: 256 rows of up to 2048 tokens in 2 kv heads 62 us with 12 or 16 heads each, 52 with 8.
 #pragma once
 #include <cuda.h>
 #include <cuda_bf16.h>

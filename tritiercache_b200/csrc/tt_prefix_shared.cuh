@@ -11,8 +11,9 @@
 // and O_t += P_t V (P from tensor memory, V from shared memory).  m is a reference that is raised, and O
 // rescaled, only when a logit exceeds it by kSlack, as in the rows' pass.
 //
-// Work: units of (kv head, row tile), each kv_tiles key tiles; the flattened list is cut into spans, one per
-// CTA, so that every SM has about the same number of tiles whatever the shape.  Where the row tiles of a
+// Work: units of (kv head, row tile), each kv_tiles key tiles.  Each unit is cut into the same number of equal spans,
+// one per CTA; where that would leave too many SMs idle the flattened list of all units' tiles is cut instead, and a
+// CTA's span may cross into the next unit (tt_prefix_plan.cuh).  Where the row tiles of a
 // kv head fill the SMs in whole groups, a group of CTAs takes the same span for all of them, so that each K
 // and V page comes from HBM once and from L2 for the rest of the group.  A span inside a unit leaves one
 // partial (m, l, O) per accumulator in the workspace, in a slot that no other span has; the join adds them.
