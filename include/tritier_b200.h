@@ -401,8 +401,8 @@ typedef enum { TT_DTYPE_F32 = 0, TT_DTYPE_BF16 = 1, TT_DTYPE_F16 = 2 } tt_dtype;
  *    for want of pages or not, but not those that do not fit a row or the table)
  *    exceed the stack; it then gets no page and its table row stays.
  *  - The step's rows are the requests' new tokens, request after request.
- *    Row i of request b: positions = ctx + i + position_offset, slots the
- *    token's slot, row_seq = b, row_lens = ctx + i + 1.  Rows of deferred
+ *    Row i of request b: positions = ctx + i + position_offset (which has to
+ *    fit int32), slots the token's slot, row_seq = b, row_lens = ctx + i + 1.  Rows of deferred
  *    requests and rows behind the last request: -1 in slots and row_seq, 0 in
  *    positions and row_lens.
  *  - seq_lens[b] = ctx + new, ctx when deferred, 0 when ended; cu_new[b] is the
